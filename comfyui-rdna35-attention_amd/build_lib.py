@@ -22,7 +22,7 @@ LIB_PATH = PACKAGE_DIR / "mi355x_pisa" / "libpisa_hip.so"
 ARCH = "gfx950"
 
 SOURCES = ("api.hip", "stats.hip", "route.hip", "attention.hip", "attention_dense.hip", "attention_d64.hip",
-           "fixed_block.hip", "layout.hip")
+           "fixed_block.hip", "layout.hip", "qk_norm_rope.hip")
 
 COMMON_FLAGS = [
     f"--offload-arch={ARCH}",

@@ -963,4 +963,159 @@ int attn_hip_fixed_block_forward(int32_t dtype, int32_t batch, int32_t heads, in
                                                causal, none, stream);
 }
 
+
+// ---- norm of queries and keys with the rotation by position
+static int fill_rope(const pisa_rope& r, int tokens, int head_dim, pisa::RopeArgs& o) {
+    memset(&o, 0, sizeof(o));
+    o.interleaved = r.interleaved ? 1 : 0;
+    o.inverse = r.inverse ? 1 : 0;
+    o.grid_h = o.grid_w = 1;
+    if (r.axes == 0) return PISA_OK;
+    if (r.axes < 0 || r.axes > PISA_ROPE_MAX_AXES)
+        return fail(PISA_ERR_INVALID_ARGUMENT, "rotation supports 1 to %d axes, got %d", PISA_ROPE_MAX_AXES, r.axes);
+    int pairs = 0;
+    for (int i = 0; i < r.axes; ++i) {
+        if (r.axis_dims[i] <= 0 || r.axis_dims[i] % 2 || r.axis_dims[i] > head_dim)
+            return fail(PISA_ERR_INVALID_ARGUMENT, "axis %d: dims must be a positive even number up to head_dim, got %d", i,
+                        r.axis_dims[i]);
+        pairs += r.axis_dims[i] / 2;
+        if (i < 3) o.axis_end[i] = pairs;
+    }
+    for (int i = r.axes; i < 3; ++i) o.axis_end[i] = pairs;
+    if (2 * pairs > head_dim || pairs % 4)
+        return fail(PISA_ERR_INVALID_ARGUMENT, "the rotated dims (%d) must be a multiple of 8 up to head_dim %d", 2 * pairs,
+                    head_dim);
+    if (!r.inv_freq || (reinterpret_cast<uintptr_t>(r.inv_freq) & 7))
+        return fail(PISA_ERR_INVALID_ARGUMENT, "inv_freq must be a non-null, 8-byte aligned array of doubles");
+    o.pairs = pairs;
+    o.inv_freq = r.inv_freq;
+    o.pos_kind = r.positions_kind;
+    if (r.positions_kind == PISA_POSITIONS_GRID) {
+        if (r.axes != 3) return fail(PISA_ERR_INVALID_ARGUMENT, "grid positions need 3 axes, got %d", r.axes);
+        if (r.grid.frames <= 0 || r.grid.height <= 0 || r.grid.width <= 0 ||
+            (int64_t)r.grid.height * r.grid.width > tokens ||
+            (int64_t)r.grid.frames * ((int64_t)r.grid.height * r.grid.width) != tokens)
+            return fail(PISA_ERR_INVALID_ARGUMENT, "token grid %dx%dx%d does not match %d tokens", r.grid.frames,
+                        r.grid.height, r.grid.width, tokens);
+        o.grid_h = r.grid.height;
+        o.grid_w = r.grid.width;
+        return PISA_OK;
+    }
+    if (r.positions_kind < PISA_POSITIONS_GRID || r.positions_kind > PISA_POSITIONS_F32)
+        return fail(PISA_ERR_INVALID_ARGUMENT, "unknown positions kind %d", r.positions_kind);
+    const int psize = r.positions_kind == PISA_POSITIONS_I64 ? 8 : 4;
+    if (!r.positions || (reinterpret_cast<uintptr_t>(r.positions) & (psize - 1)))
+        return fail(PISA_ERR_INVALID_ARGUMENT, "positions must be non-null and aligned to their element size");
+    o.pos = r.positions;
+    o.pos_sb = r.batch_stride;
+    o.pos_st = r.token_stride;
+    o.pos_sa = r.axis_stride;
+    return PISA_OK;
+}
+
+static int fill_norm_rope(const char* what, int dtype, int weight_dtype, int batch, int q_heads, int k_heads, int tokens,
+                          int head_dim, const pisa_rope& rope, float eps, pisa::NormRopeArgs& a) {
+    memset(&a, 0, sizeof(a));
+    if (dtype != PISA_DTYPE_BF16 && dtype != PISA_DTYPE_F16 && dtype != PISA_DTYPE_F32)
+        return fail(PISA_ERR_UNSUPPORTED, "%s supports bf16, fp16 and fp32", what);
+    if (weight_dtype != dtype && weight_dtype != PISA_DTYPE_F32)
+        return fail(PISA_ERR_UNSUPPORTED, "%s: weights must be of the inputs' type or fp32", what);
+    if (batch <= 0 || q_heads <= 0 || k_heads < 0 || tokens <= 0)
+        return fail(PISA_ERR_INVALID_ARGUMENT, "%s requires B>0, Hq>0, Hk>=0, T>0", what);
+    if (head_dim <= 0 || head_dim % 8 || head_dim > 256)
+        return fail(PISA_ERR_UNSUPPORTED, "%s supports head_dim a multiple of 8 up to 256, got %d", what, head_dim);
+    int rc;
+    if ((rc = check_sizes(what, batch, q_heads, tokens)) || (rc = check_sizes(what, batch, k_heads, tokens))) return rc;
+    if (!(eps >= 0.0f) || eps == __builtin_inff())
+        return fail(PISA_ERR_INVALID_ARGUMENT, "%s: eps must be finite and not negative", what);
+    if ((rc = fill_rope(rope, tokens, head_dim, a.rope))) return rc;
+    a.batch = batch;
+    a.heads[0] = q_heads;
+    a.heads[1] = k_heads;
+    a.tokens = tokens;
+    a.head_dim = head_dim;
+    a.eps = eps;
+    a.weight_f32 = weight_dtype == PISA_DTYPE_F32;
+    pisa::norm_rope_split(a);
+    return PISA_OK;
+}
+
+// Base pointer aligned to the element (the kernels need no more).
+static int check_element_view(const char* name, const pisa_view& v, int esize) {
+    if (!v.data || (reinterpret_cast<uintptr_t>(v.data) & (esize - 1)))
+        return fail(PISA_ERR_INVALID_ARGUMENT, "%s must be non-null and aligned to its element size", name);
+    return PISA_OK;
+}
+
+int attn_hip_qk_norm_rope(int32_t dtype, int32_t weight_dtype, int32_t batch, int32_t q_heads, int32_t k_heads,
+                          int32_t tokens, int32_t head_dim, pisa_view q, pisa_view k, pisa_view q_out, pisa_view k_out,
+                          const void* q_weight, const void* k_weight, int32_t normalize, float eps, pisa_rope rope,
+                          void* stream) {
+    pisa::NormRopeArgs a;
+    int rc = fill_norm_rope("qk_norm_rope", dtype, weight_dtype, batch, q_heads, k_heads, tokens, head_dim, rope, eps, a);
+    if (rc) return rc;
+    const int es = elem_size(dtype);
+    if (!normalize && (q_weight || k_weight))
+        return fail(PISA_ERR_INVALID_ARGUMENT, "weights need normalize");
+    if ((rc = check_element_view("q", q, es)) || (rc = check_element_view("q_out", q_out, es)) ||
+        (k_heads && ((rc = check_element_view("k", k, es)) || (rc = check_element_view("k_out", k_out, es)))))
+        return rc;
+    if ((rc = check_device())) return rc;
+    a.norm = normalize ? 1 : 0;
+    a.in[0] = to_view(q, q_heads);
+    a.out[0] = to_out(q_out, q_heads);
+    a.weight[0] = q_weight;
+    if (k_heads) {
+        a.in[1] = to_view(k, k_heads);
+        a.out[1] = to_out(k_out, k_heads);
+        a.weight[1] = k_weight;
+    }
+    return pisa::launch_norm_rope(dtype, a, false, static_cast<hipStream_t>(stream));
+}
+
+int64_t attn_hip_qk_norm_rope_backward_workspace_bytes(int32_t head_dim, int32_t weight_grads) {
+    if (head_dim <= 0 || head_dim > 256 || !weight_grads) return 0;
+    return (int64_t)2 * head_dim * pisa::kNormRopeParts * sizeof(float);
+}
+
+int attn_hip_qk_norm_rope_backward(int32_t dtype, int32_t weight_dtype, int32_t batch, int32_t q_heads, int32_t k_heads,
+                                   int32_t tokens, int32_t head_dim, pisa_view grad_q, pisa_view grad_k, pisa_view q,
+                                   pisa_view k, const void* q_weight, const void* k_weight, pisa_view dq, pisa_view dk,
+                                   void* dq_weight, void* dk_weight, float eps, pisa_rope rope, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+    pisa::NormRopeArgs a;
+    int rc = fill_norm_rope("qk_norm_rope_backward", dtype, weight_dtype, batch, q_heads, k_heads, tokens, head_dim, rope,
+                            eps, a);
+    if (rc) return rc;
+    const int es = elem_size(dtype);
+    if ((rc = check_element_view("grad_q", grad_q, es)) || (rc = check_element_view("q", q, es)) ||
+        (rc = check_element_view("dq", dq, es)) ||
+        (k_heads && ((rc = check_element_view("grad_k", grad_k, es)) || (rc = check_element_view("k", k, es)) ||
+                     (rc = check_element_view("dk", dk, es)))))
+        return rc;
+    if (!k_heads) dk_weight = nullptr;
+    const bool weights = dq_weight || dk_weight;
+    const int64_t need = attn_hip_qk_norm_rope_backward_workspace_bytes(head_dim, weights);
+    if (weights && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need))
+        return fail(PISA_ERR_WORKSPACE, "workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)need,
+                    (long long)workspace_bytes);
+    if ((rc = check_device())) return rc;
+    a.norm = 1;
+    a.rope.inverse = !a.rope.inverse;
+    a.in[0] = to_view(q, q_heads);
+    a.grad[0] = to_view(grad_q, q_heads);
+    a.out[0] = to_out(dq, q_heads);
+    a.weight[0] = q_weight;
+    a.weight_grad[0] = dq_weight;
+    if (k_heads) {
+        a.in[1] = to_view(k, k_heads);
+        a.grad[1] = to_view(grad_k, k_heads);
+        a.out[1] = to_out(dk, k_heads);
+        a.weight[1] = k_weight;
+        a.weight_grad[1] = dk_weight;
+    }
+    a.partial = weights ? static_cast<float*>(workspace) : nullptr;
+    return pisa::launch_norm_rope(dtype, a, true, static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

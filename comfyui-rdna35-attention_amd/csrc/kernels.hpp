@@ -245,4 +245,37 @@ int launch_merge(int dtype, const char* exact, const float* exact_lse, const cha
                  const float* corr, char* out, TokenMap map, int tokens, int head_dim, int heads, int bh_count,
                  hipStream_t stream);
 
+
+// Norm of queries and keys with the rotation by position (qk_norm_rope.hip).
+struct RopeArgs {
+    const double* inv_freq;  // [pairs]
+    const void* pos;
+    int pos_kind;            // PISA_POSITIONS_*
+    int64_t pos_sb, pos_st, pos_sa;
+    int grid_h, grid_w;
+    int pairs;               // 0: no rotation
+    int axis_end[3];         // first pair past axis 0, 1, 2
+    int interleaved, inverse;
+};
+struct NormRopeArgs {
+    View in[2], grad[2];     // grad: of the outputs (backward)
+    OutView out[2];          // outputs, or gradients of the inputs (backward)
+    const void* weight[2];   // nullable
+    void* weight_grad[2];    // nullable (backward)
+    float* partial;          // [2][head_dim][norm_rope_parts] (backward; null: no weight gradient)
+    int weight_f32;
+    int norm;
+    float eps;
+    int heads[2], batch, tokens, head_dim;
+    RopeArgs rope;
+    // set by norm_rope_split
+    int rows_per_group, groups_per_token;
+    int64_t groups;
+};
+constexpr int kNormRopeParts = 1024;
+int norm_rope_lanes(int head_dim);
+void norm_rope_split(NormRopeArgs& g);
+int norm_rope_parts(const NormRopeArgs& g);
+int launch_norm_rope(int dtype, const NormRopeArgs& g, bool backward, hipStream_t stream);
+
 }  // namespace pisa

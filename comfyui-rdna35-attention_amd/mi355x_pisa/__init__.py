@@ -879,12 +879,15 @@ class _NativeNamespace:
 
 _C = _NativeNamespace()
 
+from .rotary import axial_rope, qk_norm_rope, qk_norm_rope_backward, rope_frequencies  # noqa: E402  (uses the helpers above)
+
 __all__ = [
     "BLOCK_SIZE",
     "HEAD_DIM",
     "MAX_BLOCKS",
     "SPATIAL_SPARSE_EXACT_BLOCKS",
     "SPATIAL_TOKENS",
+    "axial_rope",
     "block_stats_hyd",
     "build_info",
     "capabilities",
@@ -898,5 +901,8 @@ __all__ = [
     "generic_forward",
     "generic_stats_mode",
     "prepare",
+    "qk_norm_rope",
+    "qk_norm_rope_backward",
+    "rope_frequencies",
     "route_topk",
 ]

@@ -32,6 +32,10 @@ MASK_BOOL = 1
 MASK_ADD_F32 = 2
 MASK_ADD_F16 = 3
 MASK_ADD_BF16 = 4
+POSITIONS_GRID = 0
+POSITIONS_I32 = 1
+POSITIONS_I64 = 2
+POSITIONS_F32 = 3
 NOALLOC_SCRATCH_BYTES = 192 << 20  # static scratch of pisa_hip_forward_noalloc
 
 _DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
@@ -60,6 +64,22 @@ class PisaMask(ctypes.Structure):
 
 class PisaTokenGrid(ctypes.Structure):
     _fields_ = [("frames", ctypes.c_int32), ("height", ctypes.c_int32), ("width", ctypes.c_int32)]
+
+
+class PisaRope(ctypes.Structure):
+    _fields_ = [
+        ("inv_freq", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("axis_stride", ctypes.c_int64),
+        ("grid", PisaTokenGrid),
+        ("positions_kind", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("axis_dims", ctypes.c_int32 * 4),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+    ]
 
 
 _i32 = ctypes.c_int32
@@ -127,6 +147,17 @@ _SIGNATURES = {
     "attn_hip_fixed_block_forward_masked": (
         ctypes.c_int,
         [_i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, _f32, _i32, PisaMask, _vp],
+    ),
+    "attn_hip_qk_norm_rope": (
+        ctypes.c_int,
+        [_i32, _i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, _vp, _vp, _i32, _f32,
+         PisaRope, _vp],
+    ),
+    "attn_hip_qk_norm_rope_backward_workspace_bytes": (_i64, [_i32, _i32]),
+    "attn_hip_qk_norm_rope_backward": (
+        ctypes.c_int,
+        [_i32, _i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, _vp, _vp, PisaView, PisaView,
+         _vp, _vp, _f32, PisaRope, _vp, _i64, _vp],
     ),
 }
 

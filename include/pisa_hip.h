@@ -339,6 +339,76 @@ PISA_HIP_EXPORT int attn_hip_fixed_block_forward_masked(int32_t dtype, int32_t b
                                         pisa_view v, pisa_view out, float scale, int32_t causal,
                                         pisa_mask mask, void* stream);
 
+/* ---- norm of queries and keys with the rotation by position --------------- */
+
+/*
+ * Rotary positions with up to four axes.  Pair p of a row (p < R/2, R the sum
+ * of axis_dims) is turned by the angle position[axis(p)] * inv_freq[p]; axis 0
+ * holds the first axis_dims[0]/2 pairs, axis 1 the next, and so on.  Pair p is
+ * dims (2p, 2p+1) if interleaved, else (p, p + R/2); dims R.. are not turned.
+ * Angles are formed in fp64.  axes == 0: no rotation.
+ *   axis_dims      positive even numbers, their sum R a multiple of 8, R <= head_dim
+ *   inv_freq       double [R/2]
+ *   positions_kind PISA_POSITIONS_GRID: token t stands at (frame, row, column) of
+ *                  the grid in raster order (axes == 3, frames*height*width == tokens);
+ *                  else positions holds element (b, t, axis) at b*batch_stride +
+ *                  t*token_stride + axis*axis_stride (elements)
+ *   inverse        turn by the negative angle
+ */
+#define PISA_POSITIONS_GRID 0
+#define PISA_POSITIONS_I32 1
+#define PISA_POSITIONS_I64 2
+#define PISA_POSITIONS_F32 3
+#define PISA_ROPE_MAX_AXES 4
+typedef struct pisa_rope {
+    const double* inv_freq;
+    const void* positions;
+    int64_t batch_stride;
+    int64_t token_stride;
+    int64_t axis_stride;
+    pisa_token_grid grid;
+    int32_t positions_kind;
+    int32_t axes;
+    int32_t axis_dims[PISA_ROPE_MAX_AXES];
+    int32_t interleaved;
+    int32_t inverse;
+} pisa_rope;
+
+/*
+ * out = rotation(x * rsqrt(mean(x^2) + eps) * weight) for each row of q and k,
+ * in one launch; statistics in fp32, one rounding at the end.
+ *   dtype          bf16, fp16 or fp32 (q, k and the outputs)
+ *   weight_dtype   dtype or PISA_DTYPE_F32 (both weights)
+ *   k_heads        0: no keys (k, k_out and k_weight are not used)
+ *   head_dim       a multiple of 8 up to 256
+ *   normalize      0: the rotation alone (weights must be null)
+ *   q_weight, k_weight  [head_dim], nullable (ones)
+ * q and k have any strides (unit head_dim stride) and element alignment; the
+ * outputs may be q and k themselves, but not overlap them otherwise.
+ * No counterpart in the reference, whose models do this in torch before they
+ * call the attention override.
+ */
+PISA_HIP_EXPORT int attn_hip_qk_norm_rope(int32_t dtype, int32_t weight_dtype, int32_t batch, int32_t q_heads,
+                          int32_t k_heads, int32_t tokens, int32_t head_dim, pisa_view q, pisa_view k,
+                          pisa_view q_out, pisa_view k_out, const void* q_weight, const void* k_weight,
+                          int32_t normalize, float eps, pisa_rope rope, void* stream);
+
+/* Bytes of workspace attn_hip_qk_norm_rope_backward needs (0 without weight gradients). */
+PISA_HIP_EXPORT int64_t attn_hip_qk_norm_rope_backward_workspace_bytes(int32_t head_dim, int32_t weight_grads);
+
+/*
+ * Gradients of attn_hip_qk_norm_rope with normalize = 1 (the rotation's own
+ * gradient is attn_hip_qk_norm_rope with rope.inverse set): dq, dk from the
+ * outputs' gradients grad_q, grad_k and the forward's q, k, weights and rope;
+ * dq_weight, dk_weight [head_dim] of weight_dtype, nullable.  Sums over rows
+ * are taken in a fixed order.
+ */
+PISA_HIP_EXPORT int attn_hip_qk_norm_rope_backward(int32_t dtype, int32_t weight_dtype, int32_t batch, int32_t q_heads,
+                          int32_t k_heads, int32_t tokens, int32_t head_dim, pisa_view grad_q, pisa_view grad_k,
+                          pisa_view q, pisa_view k, const void* q_weight, const void* k_weight, pisa_view dq,
+                          pisa_view dk, void* dq_weight, void* dk_weight, float eps, pisa_rope rope,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
