@@ -22,7 +22,8 @@ LIB_PATH = PACKAGE_DIR / "mi355x_pisa" / "libpisa_hip.so"
 ARCH = "gfx950"
 
 SOURCES = ("api.hip", "stats.hip", "route.hip", "attention.hip", "attention_dense.hip", "attention_d64.hip",
-           "fixed_block.hip", "layout.hip", "qk_norm_rope.hip")
+           "fixed_block.hip", "layout.hip", "qk_norm_rope.hip",
+           "attention_train.hip", "attention_backward.hip")
 
 COMMON_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -52,7 +53,8 @@ COMMON_FLAGS = [
 # Per-source additions: the dense attention kernels (attention_dense.hip) are
 # scheduled by LLVM's max-memory-clause strategy, which measured 1.6 % faster
 # on them than the default and slower on the sparse kernels.
-EXTRA_FLAGS = {"attention_dense.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"]}
+EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"]
+               for name in ("attention_dense.hip", "attention_train.hip")}
 
 
 def flags_for(name: str) -> list[str]:

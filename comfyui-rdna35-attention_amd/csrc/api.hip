@@ -1118,4 +1118,154 @@ int attn_hip_qk_norm_rope_backward(int32_t dtype, int32_t weight_dtype, int32_t 
     return pisa::launch_norm_rope(dtype, a, true, static_cast<hipStream_t>(stream));
 }
 
+
+// ---- training: dense attention with the rows' log sums, and its backward pass
+static int check_train(const char* what, int dtype, int batch, int heads, int kv_heads, int q_tokens, int kv_tokens,
+                       int head_dim, float scale, const int32_t* kv_lengths) {
+    if (!valid_dtype(dtype)) return fail(PISA_ERR_UNSUPPORTED, "%s supports bf16 and fp16 only", what);
+    if (batch <= 0 || heads <= 0 || kv_heads <= 0 || q_tokens <= 0 || kv_tokens <= 0)
+        return fail(PISA_ERR_INVALID_ARGUMENT, "%s requires B>0, H>0, Hkv>0, Tq>0, Tk>0", what);
+    if (heads % kv_heads)
+        return fail(PISA_ERR_INVALID_ARGUMENT, "%s: %d key heads do not divide %d query heads", what, kv_heads, heads);
+    int rc;
+    if ((rc = check_sizes(what, batch, heads, q_tokens)) || (rc = check_sizes(what, batch, heads, kv_tokens))) return rc;
+    const int padded = pisa::padded_head_dim(head_dim);
+    if (!padded)
+        return fail(PISA_ERR_UNSUPPORTED, "%s supports head_dim a multiple of 8 up to 256, got %d", what, head_dim);
+    if (!(scale > 0.0f) || scale == __builtin_inff()) return fail(PISA_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+    // 32-bit byte offsets inside one head's packed tables
+    const int64_t head_table_bytes = ((int64_t)kv_tokens + pisa::kBlock - 1) / pisa::kBlock * pisa::kBlock * padded * 2;
+    if (head_table_bytes > INT32_MAX)
+        return fail(PISA_ERR_UNSUPPORTED, "%s: Tk=%d at head_dim %d needs %lld bytes of packed keys per head, above 2 GiB",
+                    what, kv_tokens, head_dim, (long long)head_table_bytes);
+    if (reinterpret_cast<uintptr_t>(kv_lengths) & 3)
+        return fail(PISA_ERR_INVALID_ARGUMENT, "kv_lengths must be aligned to 4 bytes");
+    return PISA_OK;
+}
+
+int attn_hip_dense_forward_lse(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens,
+                               int32_t kv_tokens, int32_t head_dim, pisa_view q, pisa_view k, pisa_view v, pisa_view out,
+                               float* lse, const int32_t* kv_lengths, float scale, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+    int rc = check_train("dense_forward_lse", dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, scale, kv_lengths);
+    if (rc) return rc;
+    if ((rc = check_view("q", q, 2, true)) || (rc = check_view("k", k, 2, true)) || (rc = check_view("v", v, 2, true)) ||
+        (rc = check_view("out", out, 2, true)))
+        return rc;
+    if (!lse || (reinterpret_cast<uintptr_t>(lse) & 3))
+        return fail(PISA_ERR_INVALID_ARGUMENT, "lse must be non-null and aligned to 4 bytes");
+    const int64_t need = attn_hip_dense_workspace_bytes(batch, kv_heads, kv_tokens, head_dim);
+    if (!workspace_ok(workspace, workspace_bytes, need))
+        return fail(PISA_ERR_WORKSPACE, "workspace of %lld bytes required, got %lld", (long long)need,
+                    (long long)workspace_bytes);
+    if ((rc = check_device())) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int padded = pisa::padded_head_dim(head_dim);
+    const int kv_blocks = (kv_tokens + pisa::kBlock - 1) / pisa::kBlock;
+    char* kp = static_cast<char*>(workspace);
+    char* vp = kp + need / 2;
+    pisa::AttnTrainArgs aa;
+    memset(&aa, 0, sizeof(aa));
+    aa.q = to_view(q, heads);
+    aa.o = to_out(out, heads);
+    aa.kp = kp;
+    aa.vp = vp;
+    aa.qmap = pisa::TokenMap{0, 0, 0};
+    aa.q_tokens = q_tokens;
+    aa.kv_tokens = kv_tokens;
+    aa.q_blocks = (q_tokens + pisa::kBlock - 1) / pisa::kBlock;
+    aa.kv_blocks = kv_blocks;
+    aa.scale_log2 = scale * pisa::kLog2e;
+    aa.inv_scale_log2 = 1.0f / aa.scale_log2;
+    aa.head_dim = head_dim;
+    aa.lse = lse;
+    aa.kv_lengths = kv_lengths;
+    aa.kv_group = heads / kv_heads;
+    const pisa::View kv = to_view(k, kv_heads), vv = to_view(v, kv_heads);
+    const int kv_bh = batch * kv_heads;
+    if (kv_lengths)
+        rc = pisa::launch_kv_pack_lengths(dtype, padded, head_dim, kv, vv, kv_lengths, kv_tokens, kv_blocks, kv_bh, kp, vp, st);
+    else
+        rc = pisa::launch_kv_pack(dtype, padded, head_dim, kv, vv, aa.qmap, kv_tokens, kv_blocks, kv_bh, kp, vp, st);
+    if (rc) return rc;
+    return pisa::launch_attention_train(dtype, padded, aa, batch * heads, st);
+}
+
+static int64_t carve_backward(int dtype, int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int head_dim,
+                              void* workspace, pisa::BackwardArgs& a) {
+    const pisa::BackwardPlan p = pisa::plan_backward(batch, heads, kv_heads, q_tokens, kv_tokens,
+                                                     pisa::padded_head_dim(head_dim), dtype == PISA_DTYPE_F16);
+    a.q_units = p.q_units;
+    a.kv_units = p.kv_units;
+    a.q_parts = p.q_parts;
+    a.kv_parts = p.kv_parts;
+    Carver c(workspace);
+    a.qx = c.take<char>(p.qx_bytes);
+    a.kx = c.take<char>(p.kx_bytes);
+    a.q_most = c.take<float>(p.q_most_bytes);
+    a.v_most = c.take<float>(p.v_most_bytes);
+    a.l_most = c.take<float>(p.l_most_bytes);
+    a.part = c.take<float>(p.part_bytes);
+    return c.off;
+}
+
+int64_t attn_hip_dense_backward_workspace_bytes(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads,
+                                                int32_t q_tokens, int32_t kv_tokens, int32_t head_dim) {
+    if (check_train("dense_backward", dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, 1.0f, nullptr)) return 0;
+    pisa::BackwardArgs a;
+    memset(&a, 0, sizeof(a));
+    return carve_backward(dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, nullptr, a);
+}
+
+int attn_hip_dense_backward(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens,
+                            int32_t kv_tokens, int32_t head_dim, pisa_view q, pisa_view k, pisa_view v, pisa_view out,
+                            pisa_view grad_out, const float* lse, const float* grad_lse, const int32_t* kv_lengths,
+                            float scale, pisa_view dq, pisa_view dk, pisa_view dv, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    int rc = check_train("dense_backward", dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, scale, kv_lengths);
+    if (rc) return rc;
+    if (!dq.data && !dk.data && !dv.data) return fail(PISA_ERR_INVALID_ARGUMENT, "dq, or dk and dv, must be given");
+    if (!dk.data != !dv.data) return fail(PISA_ERR_INVALID_ARGUMENT, "dk and dv go together");
+    if ((rc = check_view("q", q, 2, true)) || (rc = check_view("k", k, 2, true)) || (rc = check_view("v", v, 2, true)) ||
+        (rc = check_view("out", out, 2, true)) || (rc = check_view("grad_out", grad_out, 2, true)) ||
+        (dq.data && (rc = check_view("dq", dq, 2, true))) ||
+        (dk.data && ((rc = check_view("dk", dk, 2, true)) || (rc = check_view("dv", dv, 2, true)))))
+        return rc;
+    if (!lse || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(grad_lse) & 3))
+        return fail(PISA_ERR_INVALID_ARGUMENT, "lse must be non-null, lse and grad_lse aligned to 4 bytes");
+    // the packing launch has a workgroup for every 64-row block of both sides
+    const int64_t blocks = (int64_t)batch * heads * (((int64_t)q_tokens + 63) / 64) +
+                           (int64_t)batch * kv_heads * (((int64_t)kv_tokens + 63) / 64);
+    if (blocks > kMaxGridBlocks)
+        return fail(PISA_ERR_UNSUPPORTED, "dense_backward supports %lld 64-row blocks of queries and keys over all heads, got %lld",
+                    (long long)kMaxGridBlocks, (long long)blocks);
+    pisa::BackwardArgs a;
+    memset(&a, 0, sizeof(a));
+    const int64_t need = carve_backward(dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, workspace, a);
+    if (!workspace_ok(workspace, workspace_bytes, need))
+        return fail(PISA_ERR_WORKSPACE, "workspace of %lld bytes required, got %lld", (long long)need,
+                    (long long)workspace_bytes);
+    if ((rc = check_device())) return rc;
+    a.q = to_view(q, heads);
+    a.k = to_view(k, kv_heads);
+    a.v = to_view(v, kv_heads);
+    a.o = to_view(out, heads);
+    a.dout = to_view(grad_out, heads);
+    a.dq = to_out(dq, heads);
+    a.dk = to_out(dk, kv_heads);
+    a.dv = to_out(dv, kv_heads);
+    a.lse = lse;
+    a.dlse = grad_lse;
+    a.kv_lengths = kv_lengths;
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_group = heads / kv_heads;
+    a.q_tokens = q_tokens;
+    a.kv_tokens = kv_tokens;
+    a.head_dim = head_dim;
+    a.scale = scale;
+    a.scale_log2 = scale * pisa::kLog2e;
+    return pisa::launch_attention_backward(dtype, pisa::padded_head_dim(head_dim), a, static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

@@ -50,25 +50,7 @@ constexpr int kStepGeneral = 0, kStepExact = 1, kStepTail = 2;
 struct NextBlock {
     int bh, qb, sub, nt;
 };
-typedef __attribute__((address_space(3))) char lds_char;
-
-// Direct-to-LDS copy of 16 bytes per lane: lane l's 16 bytes at gptr land at
-// LDS byte address lds_base + 16 l.  Written as inline asm so that the
-// compiler's memory-counter bookkeeping does not model it (it would fall back
-// to full waits in the chunk loop); its counts then include fewer operations
-// than are in flight, which only makes its waits stricter, and the callers
-// order the copy with explicit waits.
-// M0 (the LDS base of the copy) is reserved by the compiler, which warns about
-// clobbering it; no other code in these kernels uses M0.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void lds_copy16(const void* gptr, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                 :
-                 : "v"(gptr), "s"(lds_base)
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
+template <bool TRAIN> using ArgsFor = std::conditional_t<TRAIN, AttnTrainArgs, AttnArgs>;
 
 // D is the padded head dim (padded_head_dim); a.head_dim <= D is the real
 // one.  A wave holds NT 32-row query tiles of query block qb of head bh, rows
@@ -76,8 +58,16 @@ __device__ __forceinline__ void lds_copy16(const void* gptr, uint32_t lds_base) 
 // D = 128, or one tile (NT = 1, sub = 0 or 1, two waves per block) above,
 // where the accumulators and operands of 64 rows would not fit the 512
 // registers, and for the split blocks of the last round (attention_kernel).
-template <typename T, int D, int NT, bool SPARSE, bool TAIL, bool PERSIST = false>
-__device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int qb, int sub,
+//
+// TRAIN (dense, not persistent): the forward of a training step.  Head bh reads
+// the packed tables of key head bh / kv_group, the first kv_lengths[batch] keys
+// of them, and also writes the logarithm of each row's sum of exponentials.
+// There the sum is that of the probabilities before they are rounded for the
+// second product: the backward pass forms them again from it, and a sum of
+// rounded values would be off by half a step of T where one key holds the row.
+// A batch entry with no key at all gives zero rows and minus infinity.
+template <typename T, int D, int NT, bool SPARSE, bool TAIL, bool PERSIST = false, bool TRAIN = false>
+__device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh, int qb, int sub,
                                                 const int32_t* __restrict__ sel,
                                                 const uint32_t* __restrict__ selmask,
                                                 lds_char* lds = nullptr, bool from_lds = false,
@@ -97,6 +87,12 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
     const int col = lane & 31;
     const float c = a.scale_log2;
     const bool all_dims = a.head_dim >= D;  // else dims past the real head dim read as zero
+    static_assert(!TRAIN || (!SPARSE && !TAIL && !PERSIST), "the training forward is dense");
+    int kv_tokens = a.kv_tokens, kv_bh = bh;
+    if constexpr (TRAIN) {
+        kv_bh = bh / a.kv_group;
+        if (a.kv_lengths) kv_tokens = min(max(a.kv_lengths[bh / a.q.heads], 0), kv_tokens);
+    }
 
     // Token of row r of block j is block_base(j) + intra_offset(r); this
     // wave's rows are 32(sub + nt) + col.
@@ -187,7 +183,7 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
     }
 
     // ---- chunk list: [0, n_exact) exact blocks, [n_exact, n_chunks) centroid chunks
-    const int n_exact = SPARSE ? a.exact : a.kv_blocks;
+    const int n_exact = SPARSE ? a.exact : TRAIN ? (kv_tokens + kBlock - 1) / kBlock : a.kv_blocks;
     const int n_chunks = n_exact + (TAIL ? a.npad / kBlock : 0);
     const int32_t* my_idx = SPARSE ? sel + ((int64_t)bh * a.q_blocks + qb) * a.exact : nullptr;
     const uint32_t* my_mask = TAIL ? selmask + ((int64_t)bh * a.q_blocks + qb) * a.mask_words : nullptr;
@@ -197,9 +193,9 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
     constexpr int kRawFlags = 0x00020000;  // untyped 32-bit data format
     const int tab_bytes = a.kv_blocks * (int)kBlockBytes;
     const __amdgpu_buffer_rsrc_t kp_rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)(a.kp + (int64_t)bh * a.kv_blocks * kBlockBytes), (short)0, tab_bytes, kRawFlags);
+        (void*)(a.kp + (int64_t)kv_bh * a.kv_blocks * kBlockBytes), (short)0, tab_bytes, kRawFlags);
     const __amdgpu_buffer_rsrc_t vp_rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)(a.vp + (int64_t)bh * a.kv_blocks * kBlockBytes), (short)0, tab_bytes, kRawFlags);
+        (void*)(a.vp + (int64_t)kv_bh * a.kv_blocks * kBlockBytes), (short)0, tab_bytes, kRawFlags);
     const int cen_bytes = TAIL ? a.npad * D * (int)sizeof(T) : 0;
     const __amdgpu_buffer_rsrc_t kc_rs = __builtin_amdgcn_make_buffer_rsrc(
         (void*)(TAIL ? a.kbar + (int64_t)bh * a.npad * D * sizeof(T) : a.kp), (short)0, cen_bytes, kRawFlags);
@@ -330,7 +326,7 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
     // Whether half chunks of chunk x (table row `row`) need transform_half: tail
     // chunks whose bias is not added by the matrix core, and a short last key
     // block (wave-uniform).
-    auto special = [&](int x, int row) { return (!kBiasMfma && is_tail(x)) || (row + 1) * kBlock > a.kv_tokens; };
+    auto special = [&](int x, int row) { return (!kBiasMfma && is_tail(x)) || (row + 1) * kBlock > kv_tokens; };
     // A operand of the bias MFMA of half mt of chunk x (table row `row`):
     // lane (0, col) holds the bias of centroid 64 row + 32 mt + col divided by
     // c, as bf16 hi and lo; every other slot is zero (all of them for an exact
@@ -385,11 +381,11 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
     // the factor that converts the resulting scores to log2 units.
     auto transform_half = [&](int x, int row, int mt, f32x16 (&s)[NT]) -> float {
         if (!is_tail(x)) {
-            if ((row + 1) * kBlock > a.kv_tokens) {  // wave-uniform: only a short last block
+            if ((row + 1) * kBlock > kv_tokens) {  // wave-uniform: only a short last block
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const int key = row * kBlock + mt * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
-                    if (key >= a.kv_tokens)
+                    if (key >= kv_tokens)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) s[nt][v] = -__builtin_inff();
                 }
@@ -497,7 +493,7 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
                 const vec8 bf1 = (kBiasMfma && !exact_k) ? bias_frag(cc, row0, 1) : ones_frag;
                 scores_half(kf[1], sb, (kBiasMfma && (tail_k || (!exact_k && is_tail(cc)))) ? &bf1 : nullptr);
             }
-            probs_half<T, NT>(sa, ca, nm, l, lt, tail, pf);
+            probs_half<T, NT, TRAIN>(sa, ca, nm, l, lt, tail, pf);
             load_k_half(kf[1], kn, 1);
             pv_half(0, pf);
             load_v_half(vn, 0);
@@ -508,7 +504,7 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
                 const vec8 bf0 = (kBiasMfma && !exact_k) ? bias_frag(cc + 1, row1, 0) : ones_frag;
                 scores_half(kf[0], sa, (kBiasMfma && (tail_k || (!exact_k && is_tail(cc + 1)))) ? &bf0 : nullptr);
             }
-            if (!half0_only) probs_half<T, NT>(sb, cb, nm, l, lt, tail, pf);
+            if (!half0_only) probs_half<T, NT, TRAIN>(sb, cb, nm, l, lt, tail, pf);
             load_k_half(kf[0], kn2, 0);
             if (!half0_only) pv_half(1, pf);
             load_v_half(vn, 1);
@@ -556,6 +552,12 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
         const float ltf = add_xor32(lt[nt]);
         inv[nt] = 1.0f / lf;
         wa[nt] = ltf * inv[nt] * a.corr_scale;
+        if constexpr (TRAIN) {
+            if (n_chunks == 0) inv[nt] = 0.0f;
+            const int row = qb * kBlock + 32 * (sub + nt) + col;
+            if (half == 0 && row < a.q_tokens)
+                a.lse[(int64_t)bh * a.q_tokens + row] = n_chunks == 0 ? -__builtin_inff() : (__builtin_log2f(lf) - nm[nt]) * kLn2;
+        }
     }
     char* obase[NT];
     bool ovalid[NT];
@@ -657,9 +659,9 @@ __device__ __forceinline__ void attention_block(const AttnArgs& a, int bh, int q
 // (NT = 1, ~0.6 of a block's time each) that fill the XCD's SIMDs.  Each XCD
 // takes a contiguous range of qx = B / 8 blocks: its first qx - r work items
 // are whole blocks, the following 2r the halves of the rest, dispatched last.
-template <typename T, int D, bool SPARSE, bool TAIL>
+template <typename T, int D, bool SPARSE, bool TAIL, bool TRAIN = false>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void attention_kernel(AttnArgs a, const int32_t* __restrict__ sel, const uint32_t* __restrict__ selmask) {
+void attention_kernel(ArgsFor<TRAIN> a, const int32_t* __restrict__ sel, const uint32_t* __restrict__ selmask) {
     // sel/selmask are a.idx/a.selmask passed as restrict-qualified arguments: the
     // kernel never writes them, so their wave-uniform reads become scalar loads.
     if constexpr (D == 128) {
@@ -671,12 +673,12 @@ void attention_kernel(AttnArgs a, const int32_t* __restrict__ sel, const uint32_
             if (local < full) {
                 const int blk = xcd * qx + local;
                 const int bh = blk / a.q_blocks;
-                attention_block<T, D, 2, SPARSE, TAIL>(a, bh, blk - bh * a.q_blocks, 0, sel, selmask);
+                attention_block<T, D, 2, SPARSE, TAIL, false, TRAIN>(a, bh, blk - bh * a.q_blocks, 0, sel, selmask);
             } else {
                 const int h = local - full;
                 const int blk = xcd * qx + full + (h >> 1);
                 const int bh = blk / a.q_blocks;
-                attention_block<T, D, 1, SPARSE, TAIL>(a, bh, blk - bh * a.q_blocks, h & 1, sel, selmask);
+                attention_block<T, D, 1, SPARSE, TAIL, false, TRAIN>(a, bh, blk - bh * a.q_blocks, h & 1, sel, selmask);
             }
             return;
         }
@@ -691,8 +693,8 @@ void attention_kernel(AttnArgs a, const int32_t* __restrict__ sel, const uint32_
         __shared__ __attribute__((aligned(1024))) char q_lds[D / 16 * 1024];
         qbuf = (lds_char*)q_lds;
     }
-    attention_block<T, D, NT, SPARSE, TAIL>(a, bh, block_work - bh * a.q_blocks, work - block_work * SUBS, sel,
-                                            selmask, qbuf);
+    attention_block<T, D, NT, SPARSE, TAIL, false, TRAIN>(a, bh, block_work - bh * a.q_blocks,
+                                                          work - block_work * SUBS, sel, selmask, qbuf);
 }
 
 // Persistent variant (D = 128, head dim 128, a grid that splits evenly into the
@@ -757,7 +759,10 @@ void attention_persistent_kernel(AttnArgs a, const int32_t* __restrict__ sel, co
 // all 256 threads load (63 us with four).  K and V are then read with the
 // non-temporal hint (nothing reads those rows again, and the tables written here
 // stay in the caches for the attention kernel: call 733 -> 724 us).
-template <typename T, int D, bool MEANS>
+//
+// LENGTHS (training): rows from m.kv_lengths[batch] on are packed as zero, so
+// that what stands in masked keys and values (NaN too) reaches no product.
+template <typename T, int D, bool MEANS, bool LENGTHS = false>
 __global__ __launch_bounds__(256) void kv_pack_kernel(View k, View v, TokenMap map, int kv_tokens, int kv_blocks,
                                                       int d_real, char* kp, char* vp, PackMeans m) {
     typedef typename Elem<T>::vec8 vec8;
@@ -778,6 +783,8 @@ __global__ __launch_bounds__(256) void kv_pack_kernel(View k, View v, TokenMap m
     T* vdst = reinterpret_cast<T*>(vp) + ((int64_t)bh * kv_blocks + j) * D * kBlock;
     const int base = map.block_base(j);          // raster token of row r: base + intra_offset(r)
     const int last = kv_tokens - 1 - j * kBlock;  // rows past the end read the last token
+    int live_tokens = kv_tokens;
+    if constexpr (LENGTHS) live_tokens = min(m.kv_lengths[bh / k.heads], kv_tokens);
     float sums[3][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[0][e] = sums[1][e] = sums[2][e] = 0.0f;
@@ -790,7 +797,7 @@ __global__ __launch_bounds__(256) void kv_pack_kernel(View k, View v, TokenMap m
 #pragma unroll
         for (int rr = 0; rr < kRows; ++rr) {
             const int key = j * kBlock + r + rr;
-            live[rr] = key < kv_tokens && live_d;
+            live[rr] = key < live_tokens && live_d;
             const int tok = base + map.intra_offset(min(r + rr, last));
             const int dc = live_d ? pc * 8 : 0;
             if constexpr (MEANS) qx[rr] = load8<vec8>(m.q.data + (m.q.row(bh, tok) + dc) * sizeof(T));
@@ -883,13 +890,13 @@ static int xcd_slots() {
     return cus / 8 * 4;
 }
 
-template <typename T, int D, bool SPARSE, bool TAIL>
-int launch_attention_t(const AttnArgs& a_in, int bh_count, hipStream_t stream) {
+template <typename T, int D, bool SPARSE, bool TAIL, bool TRAIN = false>
+int launch_attention_t(const ArgsFor<TRAIN>& a_in, int bh_count, hipStream_t stream) {
     constexpr int kSubs = D <= 128 ? 1 : 2;  // waves per query block
-    AttnArgs a = a_in;
+    ArgsFor<TRAIN> a = a_in;
     a.q_blocks_total = bh_count * a.q_blocks;
     a.split_r = 0;
-    if constexpr (D == 128) {
+    if constexpr (D == 128 && !TRAIN) {
         static const int pslots = xcd_slots();
         if (a.head_dim == D && a.q_blocks_total % 8 == 0 && pslots > 0) {
             hipLaunchKernelGGL((attention_persistent_kernel<T, SPARSE, TAIL>), dim3(8 * pslots), dim3(64), 0, stream,
@@ -906,7 +913,7 @@ int launch_attention_t(const AttnArgs& a_in, int bh_count, hipStream_t stream) {
             waves = a.q_blocks_total + 8 * r;
         }
     }
-    hipLaunchKernelGGL((attention_kernel<T, D, SPARSE, TAIL>), dim3(waves), dim3(64), 0, stream, a, a.idx, a.selmask);
+    hipLaunchKernelGGL((attention_kernel<T, D, SPARSE, TAIL, TRAIN>), dim3(waves), dim3(64), 0, stream, a, a.idx, a.selmask);
     return pisa_host::check_launch("attention_kernel");
 }
 
@@ -918,7 +925,25 @@ int launch_attention_t(const AttnArgs& a_in, int bh_count, hipStream_t stream) {
 #define PISA_DENSE_INSTANCES(X) \
     X(bf16_t, 64) X(bf16_t, 96) X(bf16_t, 128) X(bf16_t, 160) X(bf16_t, 192) X(bf16_t, 256) \
     X(f16_t, 64) X(f16_t, 96) X(f16_t, 128) X(f16_t, 160) X(f16_t, 192) X(f16_t, 256)
-#ifdef PISA_ATTENTION_DENSE
+#if defined(PISA_ATTENTION_TRAIN)
+// attention_train.hip: the dense kernels' training variant, under the same scheduler
+template <typename T>
+static int launch_train_t(int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
+    switch (padded) {
+        case 64: return launch_attention_t<T, 64, false, false, true>(a, bh_count, stream);
+        case 96: return launch_attention_t<T, 96, false, false, true>(a, bh_count, stream);
+        case 128: return launch_attention_t<T, 128, false, false, true>(a, bh_count, stream);
+        case 160: return launch_attention_t<T, 160, false, false, true>(a, bh_count, stream);
+        case 192: return launch_attention_t<T, 192, false, false, true>(a, bh_count, stream);
+        case 256: return launch_attention_t<T, 256, false, false, true>(a, bh_count, stream);
+        default: return pisa_host::fail(PISA_ERR_UNSUPPORTED, "training attention: padded head dim %d", padded);
+    }
+}
+int launch_attention_train(int dtype, int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
+    if (dtype == PISA_DTYPE_BF16) return launch_train_t<bf16_t>(padded, a, bh_count, stream);
+    return launch_train_t<f16_t>(padded, a, bh_count, stream);
+}
+#elif defined(PISA_ATTENTION_DENSE)
 #define PISA_DENSE_INSTANCE(T, D) template int launch_attention_t<T, D, false, false>(const AttnArgs&, int, hipStream_t);
 PISA_DENSE_INSTANCES(PISA_DENSE_INSTANCE)
 #undef PISA_DENSE_INSTANCE
@@ -958,13 +983,13 @@ int launch_attention(int dtype, int padded, bool sparse, bool tail, const AttnAr
     return launch_attention_dt<f16_t>(padded, sparse, tail, a, bh_count, stream);
 }
 
-template <typename T, bool MEANS>
+template <typename T, bool MEANS, bool LENGTHS = false>
 int launch_kv_pack_t(int padded, int head_dim, const View& k, const View& v, TokenMap map, int kv_tokens,
                      int kv_blocks, int bh_count, char* kp, char* vp, const PackMeans& m, hipStream_t stream) {
     const dim3 grid(bh_count * kv_blocks);
 #define PISA_KV_PACK(DP)                                                                                         \
     case DP:                                                                                                     \
-        hipLaunchKernelGGL((kv_pack_kernel<T, DP, MEANS>), grid, dim3(256), 0, stream, k, v, map, kv_tokens, kv_blocks, \
+        hipLaunchKernelGGL((kv_pack_kernel<T, DP, MEANS, LENGTHS>), grid, dim3(256), 0, stream, k, v, map, kv_tokens, kv_blocks, \
                            head_dim, kp, vp, m);                                                                 \
         break;
     switch (padded) {
@@ -988,6 +1013,18 @@ int launch_kv_pack(int dtype, int padded, int head_dim, const View& k, const Vie
                                                stream);
     return launch_kv_pack_t<f16_t, false>(padded, head_dim, k, v, map, kv_tokens, kv_blocks, bh_count, kp, vp, none,
                                           stream);
+}
+
+int launch_kv_pack_lengths(int dtype, int padded, int head_dim, const View& k, const View& v, const int32_t* kv_lengths,
+                           int kv_tokens, int kv_blocks, int bh_count, char* kp, char* vp, hipStream_t stream) {
+    PackMeans m{};
+    m.kv_lengths = kv_lengths;
+    const TokenMap map{0, 0, 0};
+    if (dtype == PISA_DTYPE_BF16)
+        return launch_kv_pack_t<bf16_t, false, true>(padded, head_dim, k, v, map, kv_tokens, kv_blocks, bh_count, kp, vp, m,
+                                                     stream);
+    return launch_kv_pack_t<f16_t, false, true>(padded, head_dim, k, v, map, kv_tokens, kv_blocks, bh_count, kp, vp, m,
+                                                stream);
 }
 
 int launch_kv_pack_means(int dtype, int padded, int head_dim, const View& k, const View& v, TokenMap map, int kv_tokens,

@@ -1,0 +1,695 @@
+// The backward pass of exact attention: gradients of q, k and v from those of
+// the output, with the probabilities formed again from the rows' log sums.
+//
+//   S = scale q k^T,  P = exp(S - L),  dV = P^T dO,  dP = dO V^T,
+//   dS = P (dP - delta),  delta_i = sum_d dO_id O_id,
+//   dQ = scale dS K,  dK = scale dS^T Q
+//
+// One pass packs the operands (pack kernels), two kernels form the products:
+// attention_backward_kv_kernel dK and dV (four products), and
+// attention_backward_q_kernel dQ (three).  S and dP are formed in both: with
+// all five distinct products in one kernel, dQ would be summed over key blocks
+// by fp32 atomics, in an order (and with results) that change from run to run.
+//
+// Both kernels are one scheme.  A wave owns 32 N columns (keys or query rows)
+// whose operands it holds in registers as B operands, and streams the other
+// side in units of 32 rows through LDS, shared by the workgroup's four waves:
+//     X[row][column] = sum_d A[row][d] B[column][d]          (S and dP)
+//     G[dim][column] += sum_row A^T[dim][row] X[row][column]   (dK, dV, dQ)
+// The accumulator of the first product is the B operand of the second as it
+// stands (32x32x16: a lane holds one column), with the streamed rows in
+// swap23 order.  The packing kernels write both forms of every streamed operand
+// as 1 KB fragments, so a unit is one contiguous run of memory, copied to LDS
+// without passing through registers, two units ahead (three buffers; one ahead
+// at width 256), and read back without bank conflicts.  Per 32x32 tile of the
+// scores at width 128 the matrix core works 1024 (dK, dV) or 768 (dQ) cycles;
+// each fragment read from LDS feeds two tiles.
+//
+// A gradient dL of the log sums adds P dL to dS: delta - dL takes delta's place.
+// -L (in log2 units) and dL - delta travel with the query rows; the latter is
+// the starting value of dP's accumulator.  Packed rows past the end are zero and
+// have -L = -infinity, so they add nothing.  Masked keys are packed as zero, get
+// probability 0 in the dQ kernel and zero gradients in the other.
+//
+// Rounding: P and dS are rounded to the input type for the second product (as
+// P is in the forward pass); everything else is fp32.  In fp16 both would lose
+// their bits to its small range: P is scaled by 2^15, and dS by a power of two
+// from the bound |dP - delta + dL| <= 2 max_i |dO_i| max_j |V_j| + max_i |dL_i| of the head, which
+// puts its largest possible value just under 2^15; the gradients are scaled back in fp32.
+#include <type_traits>
+
+#include "kernels.hpp"
+
+namespace pisa {
+
+namespace {
+
+constexpr int kWaves = 4;       // waves of a workgroup, sharing the streamed units
+constexpr int kUnit = 32;       // streamed rows per step
+constexpr float kShift16 = 15;  // log2 of the factor on P in fp16
+
+template <typename T> constexpr bool kScaled = std::is_same<T, f16_t>::value;
+
+// Fragments of a unit: query side [Q rows][dO rows][Q^T][dO^T] of D/16 KB each
+// and 1 KB of -L and dL - delta (32 floats each); key side [K rows][V rows][K^T].
+template <int D> constexpr int q_unit_frags() { return 4 * (D / 16) + 1; }
+template <int D> constexpr int kv_unit_frags() { return 3 * (D / 16); }
+
+// Columns per wave / 32.  Two use a fragment read from LDS twice; above 128 the
+// accumulators and own operands of 64 columns do not fit 512 registers.
+template <int D> constexpr int columns() { return D <= 128 ? 2 : 1; }
+template <int D> constexpr int stages() { return D <= 192 ? 3 : 2; }
+
+// ---------------------------------------------------------------- packing
+// One 64-row block of X into two units: 16-byte pieces of rows (fragment lane
+// (half, row) holds dims 16t + 8half ..) straight from registers, and the
+// transposed fragments (lane (half, dim) holds the rows at positions 16s +
+// 8half .. of swap23 order) through LDS.  Rows from `live` on and dims from d_real on
+// are zero.  With `dot`, red[0][row][piece] receives the pieces of sum_d X Y;
+// with `squares`, red[1][row][piece] those of sum_d X^2.
+template <typename T, int D> struct PackLds {
+    static constexpr int kPieces = D / 8;
+    T t[D * (kBlock + 8)];
+    float red[2][kBlock][kPieces + 1];
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void pack_block(PackLds<T, D>& lds, const char* x, int64_t st, const char* y, int64_t yst,
+                                           int live, int last, int d_real, char* units, int64_t unit_bytes, int rows_at,
+                                           int trans_at, bool squares) {
+    typedef typename Elem<T>::vec8 vec8;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    constexpr int kRow = kBlock + 8;
+    constexpr int kPieces = D / 8;
+    constexpr int kGroups = 256 / kPieces;
+    const int t = threadIdx.x;
+    const int pc = t % kPieces;
+    const int r0 = t / kPieces;
+    const bool live_d = pc * 8 < d_real;
+    const int dc = live_d ? pc * 8 : 0;
+    for (int r = r0 * 4; r0 < kGroups && r < kBlock; r += kGroups * 4) {
+        vec8 xv[4], yv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // rows past the end read the last one
+            xv[i] = load8<vec8>(x + (min(r + i, last) * st + dc) * (int64_t)sizeof(T));
+            if (y) yv[i] = load8<vec8>(y + (min(r + i, last) * yst + dc) * (int64_t)sizeof(T));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (r + i >= live || !live_d) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) xv[i][e] = T(0.0f);
+                if (y) yv[i] = xv[i];
+            }
+            const int row = (r + i) & 31;
+            char* unit = units + ((r + i) >> 5) * unit_bytes;
+            if (rows_at >= 0) store8(unit + rows_at * 1024 + ((pc >> 1) * 64 + (pc & 1) * 32 + row) * 16, xv[i]);
+            float dot = 0.0f, sq = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = to_f32(xv[i][e]);
+                if (y) dot = fmaf(f, to_f32(yv[i][e]), dot);
+                sq = fmaf(f, f, sq);
+            }
+            if (y) lds.red[0][r + i][pc] = dot;
+            if (squares) lds.red[1][r + i][pc] = sq;
+        }
+        if (trans_at >= 0) {
+            const int p = (r & 32) | swap23(r & 31);  // four rows stay consecutive
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const vec4 w = {xv[0][e], xv[1][e], xv[2][e], xv[3][e]};
+                *reinterpret_cast<vec4*>(&lds.t[(pc * 8 + e) * kRow + p]) = w;
+            }
+        }
+    }
+    __syncthreads();
+    if (trans_at >= 0) {
+        for (int id = t; id < D * 8; id += 256) {  // 16-byte pieces: unit, fragment (md, s), lane
+            const int u = id / (D * 4);
+            const int f = (id % (D * 4)) >> 6;
+            const int lane = id & 63;
+            const int dim = (f >> 1) * 32 + (lane & 31);
+            const int pos = u * 32 + (f & 1) * 16 + (lane >> 5) * 8;
+            store8(units + u * unit_bytes + (trans_at + f) * 1024 + lane * 16,
+                   *reinterpret_cast<const vec8*>(&lds.t[dim * kRow + pos]));
+        }
+    }
+}
+
+// Largest sqrt of the rows' sums of squares, by the first wave.
+template <typename T, int D> __device__ __forceinline__ float largest_row(const PackLds<T, D>& lds) {
+    float s = 0.0f;
+    for (int j = 0; j < D / 8; ++j) s += lds.red[1][threadIdx.x][j];
+    s = sqrtf(s);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s = fmaxf(s, __shfl_xor(s, o));
+    return s;
+}
+
+// Workgroups [0, q_work): query blocks (Q, dO, O); the rest: key blocks (K, V).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardArgs a) {
+    constexpr int KT = D / 16;
+    __shared__ __attribute__((aligned(16))) PackLds<T, D> lds;
+    const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
+    const int q_work = a.batch * a.heads * q_blocks;
+    const int t = threadIdx.x;
+    if ((int)blockIdx.x < q_work) {
+        constexpr int64_t kBytes = q_unit_frags<D>() * 1024;
+        const int bh = blockIdx.x / q_blocks;
+        const int j = blockIdx.x - bh * q_blocks;
+        const int live = a.q_tokens - j * kBlock, last = live - 1;
+        char* units = a.qx + ((int64_t)bh * a.q_units + 2 * j) * kBytes;
+        auto rows = [&](const View& v) { return v.data + v.row(bh, (int64_t)j * kBlock) * (int64_t)sizeof(T); };
+        pack_block<T, D>(lds, rows(a.dout), a.dout.st, rows(a.o), a.o.st, live, last, a.head_dim, units, kBytes, KT, 3 * KT,
+                         kScaled<T>);
+        if (t < kBlock) {
+            float delta = 0.0f;
+            for (int i = 0; i < D / 8; ++i) delta += lds.red[0][t][i];
+            const bool valid = t < live;
+            const int64_t at = (int64_t)bh * a.q_tokens + (int64_t)j * kBlock + t;
+            const float dlse = valid && a.dlse ? a.dlse[at] : 0.0f;
+            const float nl = valid ? (kScaled<T> ? kShift16 : 0.0f) - a.lse[at] * kLog2e : -__builtin_inff();
+            float* stat = reinterpret_cast<float*>(units + (t >> 5) * kBytes + 4 * KT * 1024);
+            stat[t & 31] = nl;
+            stat[32 + (t & 31)] = dlse - delta;
+            if constexpr (kScaled<T>) {
+                const float most = largest_row<T, D>(lds);
+                float most_l = fabsf(dlse);
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) most_l = fmaxf(most_l, __shfl_xor(most_l, o));
+                if (t == 0) {
+                    a.q_most[(int64_t)bh * q_blocks + j] = most;
+                    a.l_most[(int64_t)bh * q_blocks + j] = most_l;
+                }
+            }
+        }
+        __syncthreads();
+        pack_block<T, D>(lds, rows(a.q), a.q.st, nullptr, 0, live, last, a.head_dim, units, kBytes, 0, 2 * KT, false);
+    } else {
+        constexpr int64_t kBytes = kv_unit_frags<D>() * 1024;
+        const int work = blockIdx.x - q_work;
+        const int bh = work / kv_blocks;
+        const int j = work - bh * kv_blocks;
+        const int last = a.kv_tokens - j * kBlock - 1;
+        const int live = a.length(bh / a.k.heads) - j * kBlock;
+        char* units = a.kx + ((int64_t)bh * a.kv_units + 2 * j) * kBytes;
+        auto rows = [&](const View& v) { return v.data + v.row(bh, (int64_t)j * kBlock) * (int64_t)sizeof(T); };
+        pack_block<T, D>(lds, rows(a.k), a.k.st, nullptr, 0, live, last, a.head_dim, units, kBytes, 0, 2 * KT, false);
+        pack_block<T, D>(lds, rows(a.v), a.v.st, nullptr, 0, live, last, a.head_dim, units, kBytes, KT, -1, kScaled<T>);
+        if constexpr (kScaled<T>) {
+            if (t < kBlock) {
+                const float most = largest_row<T, D>(lds);
+                if (t == 0) a.v_most[(int64_t)bh * kv_blocks + j] = most;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- streaming
+// Waits until at most N of this wave's copies are in flight and its LDS reads
+// have landed, then for the other waves.  One asm block, and a compiler
+// barrier: no LDS access moves across it.
+template <int N> __device__ __forceinline__ void stage_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// This wave's share of a unit's copy (fragments wave, wave + 4, ...; past the
+// last fragment the last one again, so that every wave has as many in flight).
+template <int FRAGS>
+__device__ __forceinline__ void copy_unit(const char* src, uint32_t lds_base, int wave, int lane) {
+#pragma unroll
+    for (int j = 0; j < (FRAGS + kWaves - 1) / kWaves; ++j) {
+        const int f = min(wave + kWaves * j, FRAGS - 1);
+        lds_copy16(src + f * 1024 + lane * 16, lds_base + f * 1024);
+    }
+}
+
+template <typename V> __device__ __forceinline__ V lds_frag(const lds_char* p) {
+    return __builtin_bit_cast(V, *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(p));
+}
+
+// log2 of the factor on dS in fp16: of the largest power of two that keeps
+// `bound` below 2^15 (0 if the bound is zero or not finite).
+__device__ __forceinline__ float shift_of(float bound) {
+    if (!(bound > 0.0f) || bound == __builtin_inff()) return 0.0f;
+    const int exponent = min(max(14 - ilogbf(bound), -60), 60);
+    return static_cast<float>(__builtin_amdgcn_readfirstlane(exponent));
+}
+
+// Largest of n values by the whole workgroup, the same in every thread.
+__device__ __forceinline__ float largest(const float* x, int n, float* scratch) {
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < n; i += 64 * kWaves) m = fmaxf(m, x[i]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const float all = fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3]));
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(all)));  // a scalar register
+}
+
+// Stores 32 dims of one row per lane pair: x[v] is dim 8(v/4) + 4half + v%4 of
+// the lane's column; a swap of the lane halves makes 16-byte stores.
+template <typename T> __device__ __forceinline__ void store_tile(T* row, int d0, int d_real, const f32x16& x, int half) {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    u32x2 w[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const vec4 y = {from_f32<T>(x[4 * g]), from_f32<T>(x[4 * g + 1]), from_f32<T>(x[4 * g + 2]), from_f32<T>(x[4 * g + 3])};
+        w[g] = __builtin_bit_cast(u32x2, y);
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        u32x4 y;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const auto r = __builtin_amdgcn_permlane32_swap(w[2 * p][j], w[2 * p + 1][j], false, false);
+            y[j] = r[0];
+            y[2 + j] = r[1];
+        }
+        const int d = d0 + 8 * (2 * p + half);
+        if (d < d_real) *reinterpret_cast<u32x4*>(row + d) = y;
+    }
+}
+
+// The gradient of one 32-column unit: to its rows, or, where the streamed side
+// is split over several workgroups, in fp32 to this part's slot (summed in order
+// by attention_backward_join_kernel).  Element (lane, v) of tile md of a slot is at
+// ((md * 4 + v / 4) * 64 + lane) * 4 + v % 4.
+template <typename T, int MD>
+__device__ __forceinline__ void store_unit(const f32x16 (&g)[MD], float factor, bool live, float* slot, T* row, bool inside,
+                                           int d_real, int lane) {
+#pragma unroll
+    for (int md = 0; md < MD; ++md) {
+        f32x16 x;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[v] = live ? g[md][v] * factor : 0.0f;
+        if (slot) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 y = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+                *reinterpret_cast<f32x4*>(slot + ((md * 4 + q) * 64 + lane) * 4) = y;
+            }
+        } else if (inside) {  // lanes l and l + 32 (one row) take the same branch
+            store_tile<T>(row, md * 32, d_real, x, lane >> 5);
+        }
+    }
+}
+
+// Sums the parts of one tensor's units in order and stores the rows; one wave
+// per (head, unit, tile).
+template <typename T, int MD>
+__global__ __launch_bounds__(64) void attention_backward_join_kernel(const float* part, int parts, int64_t part_floats,
+                                                                     int units, int tokens, int d_real, OutView out) {
+    const int lane = threadIdx.x;
+    const int md = blockIdx.x % MD;
+    const int work = blockIdx.x / MD;
+    const int bh = work / units;
+    const int unit = work - bh * units;
+    const float* src = part + ((int64_t)work * MD + md) * 1024 + lane * 4;
+    f32x16 x;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[v] = 0.0f;
+    for (int i = 0; i < parts; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 y = *reinterpret_cast<const f32x4*>(src + i * part_floats + q * 256);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * q + e] += y[e];
+        }
+    const int token = unit * kUnit + (lane & 31);
+    if (token < tokens)
+        store_tile<T>(reinterpret_cast<T*>(out.data) + out.row(bh, token), md * 32, d_real, x, lane >> 5);
+}
+
+// ---------------------------------------------------------------- dK, dV
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void attention_backward_kv_kernel(BackwardArgs a) {
+    typedef typename Elem<T>::vec8 vec8;
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = q_unit_frags<D>(), S = stages<D>();
+    constexpr int kBytes = FRAGS * 1024;
+    constexpr int kCopies = (FRAGS + kWaves - 1) / kWaves;
+    __shared__ __attribute__((aligned(1024))) char lds_buf[S * kBytes];
+    lds_char* const lds = (lds_char*)lds_buf;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int tiles = (a.kv_units + kWaves * N - 1) / (kWaves * N);
+    const int work = xcd_remap(blockIdx.x, gridDim.x);
+    const int tile = work % tiles;
+    const int part = work / tiles % a.kv_parts;
+    const int bh = work / (tiles * a.kv_parts);
+    const int batch = bh / a.k.heads;
+    const int length = a.length(batch);
+    const int unit0 = (tile * kWaves + wave) * N;
+    const float c = a.scale_log2;
+
+    // steps: the live query units of each of the group's heads, one after the other
+    const int q_live = (a.q_tokens + kUnit - 1) / kUnit;
+    const int steps = tile * kWaves * N * kUnit < length ? a.kv_group * q_live : 0;
+    const int i0 = (int)((int64_t)steps * part / a.kv_parts), i1 = (int)((int64_t)steps * (part + 1) / a.kv_parts);
+    const char* const table = a.qx + (int64_t)bh * a.kv_group * a.q_units * kBytes;  // heads bh * group ..
+    auto unit_of = [&](int i) {
+        i = min(i, i1 - 1);
+        const int h = i / q_live;
+        return table + ((int64_t)h * a.q_units + (i - h * q_live)) * kBytes;
+    };
+
+    float e = 0.0f;  // log2 of dS's factor
+    if constexpr (kScaled<T>) {
+        float* scratch = reinterpret_cast<float*>(lds_buf);
+        const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
+        const float mo = largest(a.q_most + (int64_t)bh * a.kv_group * q_blocks, a.kv_group * q_blocks, scratch);
+        const float ml = largest(a.l_most + (int64_t)bh * a.kv_group * q_blocks, a.kv_group * q_blocks, scratch);
+        const float mv = largest(a.v_most + (int64_t)bh * kv_blocks, kv_blocks, scratch);
+        e = shift_of(fmaf(2.0f * mo, mv, ml));
+        __syncthreads();
+    }
+    const float f = __builtin_amdgcn_exp2f(e - kShift16);
+
+    vec8 kf[N][KT], vf[N][KT];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const char* own = a.kx + ((int64_t)bh * a.kv_units + min(unit0 + n, a.kv_units - 1)) * (kv_unit_frags<D>() * 1024) +
+                          lane * 16;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            kf[n][t] = load8<vec8>(own + t * 1024);
+            vf[n][t] = load8<vec8>(own + (KT + t) * 1024);
+        }
+    }
+    f32x16 dk[N][MD], dv[N][MD];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int md = 0; md < MD; ++md)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) dk[n][md][v] = dv[n][md][v] = 0.0f;
+
+    if (i0 < i1) {
+        const uint32_t base = (uint32_t)(uintptr_t)lds;
+        __builtin_amdgcn_s_waitcnt(kWaitVm0);  // the own operands: only copies are in flight from here on
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) copy_unit<FRAGS>(unit_of(i0 + s), base + s * kBytes, wave, lane);
+        stage_barrier<(S - 2) * kCopies>();
+        int buf = 0;
+        for (int i = i0; i < i1; ++i) {
+            copy_unit<FRAGS>(unit_of(i + S - 1), base + (buf == 0 ? S - 1 : buf - 1) * kBytes, wave, lane);
+            const lds_char* u = lds + buf * kBytes + lane * 16;
+            const lds_char* stat = lds + buf * kBytes + 4 * KT * 1024 + half * 16;
+            f32x16 s[N], dp[N], nl, nd;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 x = lds_frag<f32x4>(stat + q * 32), y = lds_frag<f32x4>(stat + 128 + q * 32);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    nl[4 * q + z] = x[z];
+                    nd[4 * q + z] = y[z];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[n][v] = 0.0f;
+                dp[n] = nd;
+            }
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const vec8 x = lds_frag<vec8>(u + t * 1024);
+#pragma unroll
+                for (int n = 0; n < N; ++n) s[n] = mfma32(x, kf[n][t], s[n]);
+            }
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const vec8 x = lds_frag<vec8>(u + (KT + t) * 1024);
+#pragma unroll
+                for (int n = 0; n < N; ++n) dp[n] = mfma32(x, vf[n][t], dp[n]);
+            }
+            vec8 p[N][2];
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    s[n][v] = __builtin_amdgcn_exp2f(fmaf(s[n][v], c, nl[v]));
+                    p[n][v >> 3][v & 7] = from_f32<T>(s[n][v]);
+                }
+#pragma unroll
+            for (int ss = 0; ss < 2; ++ss)
+#pragma unroll
+                for (int md = 0; md < MD; ++md) {
+                    const vec8 x = lds_frag<vec8>(u + (3 * KT + md * 2 + ss) * 1024);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) dv[n][md] = mfma32(x, p[n][ss], dv[n][md]);
+                }
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    p[n][v >> 3][v & 7] = from_f32<T>(kScaled<T> ? s[n][v] * (dp[n][v] * f) : s[n][v] * dp[n][v]);
+#pragma unroll
+            for (int ss = 0; ss < 2; ++ss)
+#pragma unroll
+                for (int md = 0; md < MD; ++md) {
+                    const vec8 x = lds_frag<vec8>(u + (2 * KT + md * 2 + ss) * 1024);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) dk[n][md] = mfma32(x, p[n][ss], dk[n][md]);
+                }
+            buf = buf == S - 1 ? 0 : buf + 1;
+            stage_barrier<(S - 2) * kCopies>();
+        }
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // no copy outlives the workgroup's LDS
+    }
+    const float kfac = a.scale * __builtin_amdgcn_exp2f(-e), vfac = kScaled<T> ? __builtin_amdgcn_exp2f(-kShift16) : 1.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int unit = unit0 + n;
+        if (unit >= a.kv_units) continue;
+        const int key = unit * kUnit + col;
+        const bool inside = key < a.kv_tokens, live = key < length;
+        const int64_t at = inside ? key : 0;
+        float* slot = nullptr;
+        if (a.kv_parts > 1)
+            slot = a.part + (((int64_t)part * 2 * a.batch * a.k.heads + bh) * a.kv_units + unit) * MD * 1024;
+        store_unit<T, MD>(dk[n], kfac, live, slot, reinterpret_cast<T*>(a.dk.data) + a.dk.row(bh, at), inside, a.head_dim, lane);
+        if (slot) slot += (int64_t)a.batch * a.k.heads * a.kv_units * MD * 1024;
+        store_unit<T, MD>(dv[n], vfac, live, slot, reinterpret_cast<T*>(a.dv.data) + a.dv.row(bh, at), inside, a.head_dim, lane);
+    }
+}
+
+// ---------------------------------------------------------------- dQ
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void attention_backward_q_kernel(BackwardArgs a) {
+    typedef typename Elem<T>::vec8 vec8;
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kv_unit_frags<D>(), S = stages<D>();
+    constexpr int kBytes = FRAGS * 1024;
+    constexpr int kCopies = (FRAGS + kWaves - 1) / kWaves;
+    __shared__ __attribute__((aligned(1024))) char lds_buf[S * kBytes];
+    lds_char* const lds = (lds_char*)lds_buf;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int tiles = (a.q_units + kWaves * N - 1) / (kWaves * N);
+    const int work = xcd_remap(blockIdx.x, gridDim.x);
+    const int tile = work % tiles;
+    const int part = work / tiles % a.q_parts;
+    const int bh = work / (tiles * a.q_parts);
+    const int kv_bh = bh / a.kv_group;
+    const int length = a.length(bh / a.heads);
+    const int unit0 = (tile * kWaves + wave) * N;
+    const float c = a.scale_log2;
+    const int steps = (length + kUnit - 1) / kUnit;
+    const int i0 = (int)((int64_t)steps * part / a.q_parts), i1 = (int)((int64_t)steps * (part + 1) / a.q_parts);
+    const char* const table = a.kx + (int64_t)kv_bh * a.kv_units * kBytes;
+    auto unit_of = [&](int i) { return table + (int64_t)min(i, i1 - 1) * kBytes; };
+
+    float e = 0.0f;
+    if constexpr (kScaled<T>) {
+        float* scratch = reinterpret_cast<float*>(lds_buf);
+        const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
+        const float mo = largest(a.q_most + (int64_t)bh * q_blocks, q_blocks, scratch);
+        const float ml = largest(a.l_most + (int64_t)bh * q_blocks, q_blocks, scratch);
+        const float mv = largest(a.v_most + (int64_t)kv_bh * kv_blocks, kv_blocks, scratch);
+        e = shift_of(fmaf(2.0f * mo, mv, ml));
+        __syncthreads();
+    }
+
+    vec8 qf[N][KT], of[N][KT];
+    float nl[N], nd[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const char* own = a.qx + ((int64_t)bh * a.q_units + min(unit0 + n, a.q_units - 1)) * (q_unit_frags<D>() * 1024);
+        const float* stat = reinterpret_cast<const float*>(own + 4 * KT * 1024);
+        nl[n] = stat[col] + (kScaled<T> ? e - kShift16 : 0.0f);
+        nd[n] = stat[32 + col];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            qf[n][t] = load8<vec8>(own + t * 1024 + lane * 16);
+            of[n][t] = load8<vec8>(own + (KT + t) * 1024 + lane * 16);
+        }
+    }
+    f32x16 dq[N][MD];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int md = 0; md < MD; ++md)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) dq[n][md][v] = 0.0f;
+
+    if (i0 < i1) {
+        const uint32_t base = (uint32_t)(uintptr_t)lds;
+        __builtin_amdgcn_s_waitcnt(kWaitVm0);
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) copy_unit<FRAGS>(unit_of(i0 + s), base + s * kBytes, wave, lane);
+        stage_barrier<(S - 2) * kCopies>();
+        int buf = 0;
+        for (int i = i0; i < i1; ++i) {
+            copy_unit<FRAGS>(unit_of(i + S - 1), base + (buf == 0 ? S - 1 : buf - 1) * kBytes, wave, lane);
+            const lds_char* u = lds + buf * kBytes + lane * 16;
+            f32x16 s[N], dp[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    s[n][v] = 0.0f;
+                    dp[n][v] = nd[n];
+                }
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const vec8 x = lds_frag<vec8>(u + t * 1024);
+#pragma unroll
+                for (int n = 0; n < N; ++n) s[n] = mfma32(x, qf[n][t], s[n]);
+            }
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const vec8 x = lds_frag<vec8>(u + (KT + t) * 1024);
+#pragma unroll
+                for (int n = 0; n < N; ++n) dp[n] = mfma32(x, of[n][t], dp[n]);
+            }
+            if ((i + 1) * kUnit > length) {  // the last unit's masked keys: probability 0
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (i * kUnit + 8 * (v >> 2) + 4 * half + (v & 3) >= length)
+#pragma unroll
+                        for (int n = 0; n < N; ++n) s[n][v] = -__builtin_inff();
+            }
+            vec8 p[N][2];
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    p[n][v >> 3][v & 7] = from_f32<T>(__builtin_amdgcn_exp2f(fmaf(s[n][v], c, nl[n])) * dp[n][v]);
+#pragma unroll
+            for (int ss = 0; ss < 2; ++ss)
+#pragma unroll
+                for (int md = 0; md < MD; ++md) {
+                    const vec8 x = lds_frag<vec8>(u + (2 * KT + md * 2 + ss) * 1024);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) dq[n][md] = mfma32(x, p[n][ss], dq[n][md]);
+                }
+            buf = buf == S - 1 ? 0 : buf + 1;
+            stage_barrier<(S - 2) * kCopies>();
+        }
+        __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    }
+    const float fac = a.scale * __builtin_amdgcn_exp2f(-e);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int unit = unit0 + n;
+        if (unit >= a.q_units) continue;
+        const int row = unit * kUnit + col;
+        const bool inside = row < a.q_tokens;
+        float* slot = nullptr;
+        if (a.q_parts > 1) slot = a.part + (((int64_t)part * a.batch * a.heads + bh) * a.q_units + unit) * MD * 1024;
+        store_unit<T, MD>(dq[n], fac, true, slot, reinterpret_cast<T*>(a.dq.data) + a.dq.row(bh, inside ? row : 0), inside,
+                          a.head_dim, lane);
+    }
+}
+
+template <typename T, int D>
+int launch_t(const BackwardArgs& a, hipStream_t stream) {
+    constexpr int MD = D / 32, kTile = kWaves * columns<D>();
+    const int bh = a.batch * a.heads, kv_bh = a.batch * a.k.heads;
+    int rc;
+    hipLaunchKernelGGL((attention_backward_pack_kernel<T, D>), dim3(bh * (a.q_units / 2) + kv_bh * (a.kv_units / 2)), dim3(256),
+                       0, stream, a);
+    if ((rc = pisa_host::check_launch("attention_backward_pack_kernel"))) return rc;
+    if (a.dk.data) {
+        hipLaunchKernelGGL((attention_backward_kv_kernel<T, D>), dim3(kv_bh * a.kv_parts * ((a.kv_units + kTile - 1) / kTile)),
+                           dim3(64 * kWaves), 0, stream, a);
+        if ((rc = pisa_host::check_launch("attention_backward_kv_kernel"))) return rc;
+        if (a.kv_parts > 1) {
+            const int64_t tensor = (int64_t)kv_bh * a.kv_units * MD * 1024;
+            for (int i = 0; i < 2; ++i) {
+                hipLaunchKernelGGL((attention_backward_join_kernel<T, MD>), dim3(kv_bh * a.kv_units * MD), dim3(64), 0, stream,
+                                   a.part + i * tensor, a.kv_parts, 2 * tensor, a.kv_units, a.kv_tokens, a.head_dim,
+                                   i == 0 ? a.dk : a.dv);
+                if ((rc = pisa_host::check_launch("attention_backward_join_kernel"))) return rc;
+            }
+        }
+    }
+    if (!a.dq.data) return PISA_OK;
+    hipLaunchKernelGGL((attention_backward_q_kernel<T, D>), dim3(bh * a.q_parts * ((a.q_units + kTile - 1) / kTile)),
+                       dim3(64 * kWaves), 0, stream, a);
+    if ((rc = pisa_host::check_launch("attention_backward_q_kernel"))) return rc;
+    if (a.q_parts > 1) {
+        hipLaunchKernelGGL((attention_backward_join_kernel<T, MD>), dim3(bh * a.q_units * MD), dim3(64), 0, stream, a.part,
+                           a.q_parts, (int64_t)bh * a.q_units * MD * 1024, a.q_units, a.q_tokens, a.head_dim, a.dq);
+        rc = pisa_host::check_launch("attention_backward_join_kernel");
+    }
+    return rc;
+}
+
+template <typename T>
+int launch_d(int padded, const BackwardArgs& a, hipStream_t stream) {
+    switch (padded) {
+        case 64: return launch_t<T, 64>(a, stream);
+        case 96: return launch_t<T, 96>(a, stream);
+        case 128: return launch_t<T, 128>(a, stream);
+        case 160: return launch_t<T, 160>(a, stream);
+        case 192: return launch_t<T, 192>(a, stream);
+        case 256: return launch_t<T, 256>(a, stream);
+        default: return pisa_host::fail(PISA_ERR_UNSUPPORTED, "attention backward: padded head dim %d", padded);
+    }
+}
+
+}  // namespace
+
+// How many workgroups share the streamed side of one tile of columns: as many
+// as the 256 CUs hold beside each other, while each part keeps eight units.
+static int parts_for(int64_t workgroups, int64_t steps) {
+    constexpr int64_t kSlots = 256;
+    int64_t n = workgroups > 0 ? kSlots / workgroups : 1;
+    if (n > steps / 8) n = steps / 8;
+    return n < 1 ? 1 : static_cast<int>(n);
+}
+
+BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int padded, bool scaled) {
+    BackwardPlan p;
+    const int columns_per_tile = kWaves * (padded <= 128 ? 2 : 1);
+    p.q_units = (q_tokens + kBlock - 1) / kBlock * 2;
+    p.kv_units = (kv_tokens + kBlock - 1) / kBlock * 2;
+    const int64_t bh = (int64_t)batch * heads, kv_bh = (int64_t)batch * kv_heads;
+    p.q_parts = parts_for(bh * ((p.q_units + columns_per_tile - 1) / columns_per_tile), p.kv_units);
+    p.kv_parts = parts_for(kv_bh * ((p.kv_units + columns_per_tile - 1) / columns_per_tile),
+                           (int64_t)p.q_units * (heads / kv_heads));
+    p.qx_bytes = bh * p.q_units * (4 * (padded / 16) + 1) * 1024;
+    p.kx_bytes = kv_bh * p.kv_units * 3 * (padded / 16) * 1024;
+    p.q_most_bytes = scaled ? bh * (p.q_units / 2) * (int64_t)sizeof(float) : 0;
+    p.l_most_bytes = p.q_most_bytes;
+    p.v_most_bytes = scaled ? kv_bh * (p.kv_units / 2) * (int64_t)sizeof(float) : 0;
+    const int64_t tile_bytes = (int64_t)padded * kUnit * sizeof(float);
+    const int64_t q_part = p.q_parts > 1 ? p.q_parts * bh * p.q_units * tile_bytes : 0;
+    const int64_t kv_part = p.kv_parts > 1 ? 2 * p.kv_parts * kv_bh * p.kv_units * tile_bytes : 0;
+    p.part_bytes = q_part > kv_part ? q_part : kv_part;  // the two kernels run one after the other
+    return p;
+}
+
+int launch_attention_backward(int dtype, int padded, const BackwardArgs& a, hipStream_t stream) {
+    if (dtype == PISA_DTYPE_BF16) return launch_d<bf16_t>(padded, a, stream);
+    return launch_d<f16_t>(padded, a, stream);
+}
+
+}  // namespace pisa

@@ -113,8 +113,9 @@ __device__ __forceinline__ void rescale_to(const float (&mx)[NT], bool enable, f
 // order), and their masses: l (and lt for tail chunks) sum the rounded
 // probabilities the PV product uses, so every output row's weights sum to 1.
 // Exact chunks accumulate straight into l; tail chunks form the half's sum
-// first, which goes to both l and lt.
-template <typename T, int NT>
+// first, which goes to both l and lt.  EXACT_SUM: l sums the probabilities
+// before rounding instead (its logarithm is an output of the training forward).
+template <typename T, int NT, bool EXACT_SUM = false>
 __device__ __forceinline__ void probs_half(const f32x16 (&s)[NT], float c, const float (&nm)[NT], float (&l)[NT],
                                            float (&lt)[NT], bool tail, typename Elem<T>::vec8 (&pf)[NT][2]) {
 #pragma unroll
@@ -125,9 +126,13 @@ __device__ __forceinline__ void probs_half(const f32x16 (&s)[NT], float c, const
         for (int ss = 0; ss < 2; ++ss) {
             typename Elem<T>::vec8 p;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(__builtin_amdgcn_exp2f(fmaf(s[nt][ss * 8 + e], c, neg_m)));
+            for (int e = 0; e < 8; ++e) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[nt][ss * 8 + e], c, neg_m));
+                p[e] = from_f32<T>(x);
+                if constexpr (EXACT_SUM) rs += x;
+            }
             pf[nt][ss] = p;
-            rs = sum8(p, rs);
+            if constexpr (!EXACT_SUM) rs = sum8(p, rs);
         }
         l[nt] = tail ? l[nt] + rs : rs;
         lt[nt] = tail ? lt[nt] + rs : lt[nt];

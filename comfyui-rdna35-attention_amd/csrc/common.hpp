@@ -81,6 +81,26 @@ template <typename V> __device__ __forceinline__ void store8(void* p, V v) {
     *reinterpret_cast<u32x4*>(p) = __builtin_bit_cast(u32x4, v);
 }
 
+typedef __attribute__((address_space(3))) char lds_char;
+
+// Direct-to-LDS copy of 16 bytes per lane: lane l's 16 bytes at gptr land at
+// LDS byte address lds_base + 16 l.  Written as inline asm so that the
+// compiler's memory-counter bookkeeping does not model it (it would fall back
+// to full waits in the chunk loop); its counts then include fewer operations
+// than are in flight, which only makes its waits stricter, and the callers
+// order the copy with explicit waits.
+// M0 (the LDS base of the copy) is reserved by the compiler, which warns about
+// clobbering it; no other code in these kernels uses M0.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void lds_copy16(const void* gptr, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"(gptr), "s"(lds_base)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // Cross-lane exchanges without the LDS crossbar.  v_permlane32_swap swaps the
 // upper 32 lanes of one register with the lower 32 lanes of another, so
 // applied to two copies of x it yields {x[l], x[l ^ 32]} in every lane

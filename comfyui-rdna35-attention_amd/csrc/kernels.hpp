@@ -163,6 +163,13 @@ struct AttnArgs {
     int q_blocks_total, split_r;
 };
 
+// The training forward's arguments.
+struct AttnTrainArgs : AttnArgs {
+    float* lse;                 // [BH][q_tokens]
+    const int32_t* kv_lengths;  // [B] or null
+    int kv_group;               // query heads per key head
+};
+
 struct LayoutArgs {
     View in[3];
     char* out[3];
@@ -226,7 +233,13 @@ struct PackMeans {
     void* kbar_pad;
     void* vbar_t_pad;
     int npad;
+    const int32_t* kv_lengths;  // launch_kv_pack_lengths
 };
+// launch_kv_pack with rows from kv_lengths[batch] on packed as zero.
+int launch_kv_pack_lengths(int dtype, int padded, int head_dim, const View& k, const View& v, const int32_t* kv_lengths,
+                           int kv_tokens, int kv_blocks, int bh_count, char* kp, char* vp, hipStream_t stream);
+// Dense attention that also writes the rows' log sums (attention_train.hip).
+int launch_attention_train(int dtype, int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream);
 int launch_kv_pack_means(int dtype, int padded, int head_dim, const View& k, const View& v, TokenMap map, int kv_tokens,
                          int kv_blocks, int bh_count, char* kp, char* vp, const PackMeans& m, hipStream_t stream);
 // Fixed-block attention mask, broadcast to [B][heads][T][T] by element strides.
@@ -277,5 +290,31 @@ int norm_rope_lanes(int head_dim);
 void norm_rope_split(NormRopeArgs& g);
 int norm_rope_parts(const NormRopeArgs& g);
 int launch_norm_rope(int dtype, const NormRopeArgs& g, bool backward, hipStream_t stream);
+
+// Backward pass of dense attention (attention_backward.hip).
+struct BackwardArgs {
+    View q, k, v, o, dout;
+    OutView dq, dk, dv;         // dq, or dk and dv, may be null: not formed
+    const float* lse;           // [BH][q_tokens]
+    const float* dlse;          // its gradient, or null
+    const int32_t* kv_lengths;  // [B] or null
+    int batch, heads, kv_group, q_tokens, kv_tokens, head_dim;
+    float scale, scale_log2;
+    // plan_backward: 32-row units (an even number) and the parts of the streamed side
+    int q_units, kv_units, q_parts, kv_parts;
+    char *qx, *kx;              // packed units
+    // largest row norms of dO and V and largest |dlse| by 64-row block (fp16): [BH][q_units/2], [BHk][kv_units/2]
+    float *q_most, *v_most, *l_most;
+    float* part;                // fp32 gradients of the parts
+    __device__ __forceinline__ int length(int b) const {
+        return kv_lengths ? min(max(kv_lengths[b], 0), kv_tokens) : kv_tokens;
+    }
+};
+struct BackwardPlan {
+    int q_units, kv_units, q_parts, kv_parts;
+    int64_t qx_bytes, kx_bytes, q_most_bytes, v_most_bytes, l_most_bytes, part_bytes;
+};
+BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int padded, bool scaled);
+int launch_attention_backward(int dtype, int padded, const BackwardArgs& a, hipStream_t stream);
 
 }  // namespace pisa

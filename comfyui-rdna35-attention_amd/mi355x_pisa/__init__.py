@@ -879,7 +879,9 @@ class _NativeNamespace:
 
 _C = _NativeNamespace()
 
-from .rotary import axial_rope, qk_norm_rope, qk_norm_rope_backward, rope_frequencies  # noqa: E402  (uses the helpers above)
+# these modules use the helpers above
+from .rotary import axial_rope, qk_norm_rope, qk_norm_rope_backward, rope_frequencies  # noqa: E402
+from .dense_training import dense_attention_backward, dense_attention_with_lse  # noqa: E402
 
 __all__ = [
     "BLOCK_SIZE",
@@ -893,6 +895,8 @@ __all__ = [
     "capabilities",
     "clear_compile_cache",
     "dense_attention",
+    "dense_attention_backward",
+    "dense_attention_with_lse",
     "fixed_block_attention",
     "forward",
     "forward_spatial_bhtd",

@@ -148,6 +148,16 @@ _SIGNATURES = {
         ctypes.c_int,
         [_i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, _f32, _i32, PisaMask, _vp],
     ),
+    "attn_hip_dense_forward_lse": (
+        ctypes.c_int,
+        [_i32, _i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, _vp, _vp, _f32, _vp, _i64, _vp],
+    ),
+    "attn_hip_dense_backward_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "attn_hip_dense_backward": (
+        ctypes.c_int,
+        [_i32, _i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, PisaView, _vp, _vp, _vp, _f32,
+         PisaView, PisaView, PisaView, _vp, _i64, _vp],
+    ),
     "attn_hip_qk_norm_rope": (
         ctypes.c_int,
         [_i32, _i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, _vp, _vp, _i32, _f32,

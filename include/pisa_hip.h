@@ -339,6 +339,43 @@ PISA_HIP_EXPORT int attn_hip_fixed_block_forward_masked(int32_t dtype, int32_t b
                                         pisa_view v, pisa_view out, float scale, int32_t causal,
                                         pisa_mask mask, void* stream);
 
+/* ---- training: exact attention and its backward pass ---------------------- */
+
+/*
+ * attn_hip_dense_forward that also writes lse [B*H, Tq] fp32, the natural
+ * logarithm of each row's sum of exponentials of the scaled scores.
+ *   kv_heads    divides heads: query heads h*heads/kv_heads .. share key head h
+ *   kv_lengths  nullable int32 [B] on the device: keys from kv_lengths[b] on are
+ *               masked (values are taken into [0, Tk]); what stands in them is
+ *               not used.  With no key left a row is 0 and its lse minus infinity
+ * Every view is 16-byte aligned with strides a multiple of 8 elements; the
+ * workspace is attn_hip_dense_workspace_bytes of kv_heads heads.
+ * No counterpart in the reference, which is forward-only.
+ */
+PISA_HIP_EXPORT int attn_hip_dense_forward_lse(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads,
+                               int32_t q_tokens, int32_t kv_tokens, int32_t head_dim, pisa_view q, pisa_view k,
+                               pisa_view v, pisa_view out, float* lse, const int32_t* kv_lengths, float scale,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace attn_hip_dense_backward needs (0 for problems it refuses). */
+PISA_HIP_EXPORT int64_t attn_hip_dense_backward_workspace_bytes(int32_t dtype, int32_t batch, int32_t heads,
+                                                int32_t kv_heads, int32_t q_tokens, int32_t kv_tokens,
+                                                int32_t head_dim);
+
+/*
+ * Gradients of attn_hip_dense_forward_lse from those of its outputs: grad_out,
+ * and grad_lse [B*H, Tq] (nullable: zero).  q, k, v, kv_lengths and scale are the
+ * forward's, out and lse what it wrote.  dq, or dk and dv, may have null data and
+ * are then not formed.  Masked keys get zero gradients.  The sums of dk and dv over
+ * a group's query heads and every other sum are taken in a fixed order: the
+ * result is the same bit for bit from run to run.
+ */
+PISA_HIP_EXPORT int attn_hip_dense_backward(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads,
+                            int32_t q_tokens, int32_t kv_tokens, int32_t head_dim, pisa_view q, pisa_view k,
+                            pisa_view v, pisa_view out, pisa_view grad_out, const float* lse, const float* grad_lse,
+                            const int32_t* kv_lengths, float scale, pisa_view dq, pisa_view dk, pisa_view dv,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- norm of queries and keys with the rotation by position --------------- */
 
 /*
