@@ -50,11 +50,15 @@ COMMON_FLAGS = [
 ]
 
 
-# Per-source additions: the dense attention kernels (attention_dense.hip) are
-# scheduled by LLVM's max-memory-clause strategy, which measured 1.6 % faster
-# on them than the default and slower on the sparse kernels.
+# Per-source additions: the dense attention kernels (attention_dense.hip and
+# their training variant) are scheduled by LLVM's max-memory-clause strategy,
+# which measured 1.6 % faster on them than the default and slower on the sparse
+# kernels.  The backward kernels are scheduled by their source; AMDGPU's own
+# register pressure trackers leave 64 copies between the register files in the
+# loop over units of dK and dV instead of 103, and no kernel of theirs spills.
 EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"]
                for name in ("attention_dense.hip", "attention_train.hip")}
+EXTRA_FLAGS["attention_backward.hip"] = ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"]
 
 
 def flags_for(name: str) -> list[str]:

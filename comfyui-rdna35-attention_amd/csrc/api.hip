@@ -1197,8 +1197,8 @@ static int64_t carve_backward(int dtype, int batch, int heads, int kv_heads, int
                                                      pisa::padded_head_dim(head_dim), dtype == PISA_DTYPE_F16);
     a.q_units = p.q_units;
     a.kv_units = p.kv_units;
-    a.q_parts = p.q_parts;
-    a.kv_parts = p.kv_parts;
+    a.q_tiles = p.q_tiles;
+    a.kv_tiles = p.kv_tiles;
     Carver c(workspace);
     a.qx = c.take<char>(p.qx_bytes);
     a.kx = c.take<char>(p.kx_bytes);

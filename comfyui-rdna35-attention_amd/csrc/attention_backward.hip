@@ -37,6 +37,7 @@
 // from the bound |dP - delta + dL| <= 2 max_i |dO_i| max_j |V_j| + max_i |dL_i| of the head, which
 // puts its largest possible value just under 2^15; the gradients are scaled back in fp32.
 #include <type_traits>
+#include <utility>
 
 #include "kernels.hpp"
 
@@ -50,7 +51,7 @@ constexpr float kShift16 = 15;  // log2 of the factor on P in fp16
 
 template <typename T> constexpr bool kScaled = std::is_same<T, f16_t>::value;
 
-// Fragments of a unit: query side [Q rows][dO rows][Q^T][dO^T] of D/16 KB each
+// Fragments of a unit, in the order in which they are used: query side [Q rows][dO rows][dO^T][Q^T] of D/16 KB each
 // and 1 KB of -L and dL - delta (32 floats each); key side [K rows][V rows][K^T].
 template <int D> constexpr int q_unit_frags() { return 4 * (D / 16) + 1; }
 template <int D> constexpr int kv_unit_frags() { return 3 * (D / 16); }
@@ -59,6 +60,9 @@ template <int D> constexpr int kv_unit_frags() { return 3 * (D / 16); }
 // accumulators and own operands of 64 columns do not fit 512 registers.
 template <int D> constexpr int columns() { return D <= 128 ? 2 : 1; }
 template <int D> constexpr int stages() { return D <= 192 ? 3 : 2; }
+// At width 128 the values of a wave's second 32 keys stay in LDS (read again for
+// every unit): with them the kernel would need more than 512 registers.
+template <int D> constexpr bool kValuesInLds = D == 128;
 
 // ---------------------------------------------------------------- packing
 // One 64-row block of X into two units: 16-byte pieces of rows (fragment lane
@@ -125,12 +129,12 @@ __device__ __forceinline__ void pack_block(PackLds<T, D>& lds, const char* x, in
     }
     __syncthreads();
     if (trans_at >= 0) {
-        for (int id = t; id < D * 8; id += 256) {  // 16-byte pieces: unit, fragment (md, s), lane
+        for (int id = t; id < D * 8; id += 256) {  // 16-byte pieces: unit, fragment (s, md), lane
             const int u = id / (D * 4);
             const int f = (id % (D * 4)) >> 6;
             const int lane = id & 63;
-            const int dim = (f >> 1) * 32 + (lane & 31);
-            const int pos = u * 32 + (f & 1) * 16 + (lane >> 5) * 8;
+            const int dim = f % (D / 32) * 32 + (lane & 31);
+            const int pos = u * 32 + f / (D / 32) * 16 + (lane >> 5) * 8;
             store8(units + u * unit_bytes + (trans_at + f) * 1024 + lane * 16,
                    *reinterpret_cast<const vec8*>(&lds.t[dim * kRow + pos]));
         }
@@ -162,7 +166,7 @@ __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardAr
         const int live = a.q_tokens - j * kBlock, last = live - 1;
         char* units = a.qx + ((int64_t)bh * a.q_units + 2 * j) * kBytes;
         auto rows = [&](const View& v) { return v.data + v.row(bh, (int64_t)j * kBlock) * (int64_t)sizeof(T); };
-        pack_block<T, D>(lds, rows(a.dout), a.dout.st, rows(a.o), a.o.st, live, last, a.head_dim, units, kBytes, KT, 3 * KT,
+        pack_block<T, D>(lds, rows(a.dout), a.dout.st, rows(a.o), a.o.st, live, last, a.head_dim, units, kBytes, KT, 2 * KT,
                          kScaled<T>);
         if (t < kBlock) {
             float delta = 0.0f;
@@ -186,7 +190,7 @@ __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardAr
             }
         }
         __syncthreads();
-        pack_block<T, D>(lds, rows(a.q), a.q.st, nullptr, 0, live, last, a.head_dim, units, kBytes, 0, 2 * KT, false);
+        pack_block<T, D>(lds, rows(a.q), a.q.st, nullptr, 0, live, last, a.head_dim, units, kBytes, 0, 3 * KT, false);
     } else {
         constexpr int64_t kBytes = kv_unit_frags<D>() * 1024;
         const int work = blockIdx.x - q_work;
@@ -208,22 +212,60 @@ __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardAr
 }
 
 // ---------------------------------------------------------------- streaming
-// Waits until at most N of this wave's copies are in flight and its LDS reads
-// have landed, then for the other waves.  One asm block, and a compiler
-// barrier: no LDS access moves across it.
-template <int N> __device__ __forceinline__ void stage_barrier() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+// f(0), f(1), ..., f(N - 1) with the index as a compile-time constant: the steps
+// of a unit differ in what they overlap, and loops with bounds that depend on
+// an outer unrolled index are not unrolled by the compiler.
+template <class F, int... I>
+__device__ __forceinline__ void unrolled(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F> __device__ __forceinline__ void unrolled(F&& f) {
+    unrolled(f, std::make_integer_sequence<int, N>{});
 }
 
-// This wave's share of a unit's copy (fragments wave, wave + 4, ...; past the
-// last fragment the last one again, so that every wave has as many in flight).
-template <int FRAGS>
-__device__ __forceinline__ void copy_unit(const char* src, uint32_t lds_base, int wave, int lane) {
+// Waits until this wave's copies and LDS reads have landed, then for the other
+// waves.  One asm block, and a compiler barrier: no LDS access moves across it.
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+}
+
+// This wave's share of a unit's copy to LDS (fragments wave, wave + 4, ...; past
+// the last fragment the last one again, so that every wave has as many in flight).
+// As lds_copy16, with the source address as a scalar base and a lane offset: no
+// vector register or instruction per copy.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// Fragments from SPLIT on come from `src1`.
+template <int FRAGS, int SPLIT>
+__device__ __forceinline__ void copy_unit(const char* src0, const char* src1, uint32_t lds_base, int wave,
+                                          uint32_t lane_off) {
 #pragma unroll
     for (int j = 0; j < (FRAGS + kWaves - 1) / kWaves; ++j) {
         const int f = min(wave + kWaves * j, FRAGS - 1);
-        lds_copy16(src + f * 1024 + lane * 16, lds_base + f * 1024);
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     :
+                     : "v"(lane_off), "s"((f < SPLIT ? src0 : src1) + f * 1024), "s"(lds_base + f * 1024)
+                     : "memory", "m0");
     }
+}
+#pragma clang diagnostic pop
+template <int FRAGS>
+__device__ __forceinline__ void copy_unit(const char* src, uint32_t lds_base, int wave, uint32_t lane_off) {
+    copy_unit<FRAGS, FRAGS>(src, src, lds_base, wave, lane_off);
+}
+
+// Pins the own operands to AGPRs (an empty asm with an "a" operand): the matrix
+// core reads its B operand there directly, and the architectural registers are
+// left to what the vector instructions touch.
+template <typename V, int N, int KT> __device__ __forceinline__ void pin_all(V (&frags)[N][KT]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            f32x4 x = __builtin_bit_cast(f32x4, frags[n][t]);
+            asm volatile("" : "+a"(x));
+            frags[n][t] = __builtin_bit_cast(V, x);
+        }
 }
 
 template <typename V> __device__ __forceinline__ V lds_frag(const lds_char* p) {
@@ -275,6 +317,20 @@ template <typename T> __device__ __forceinline__ void store_tile(T* row, int d0,
     }
 }
 
+// The tiles of a launch (kWaves N units of one head each): the first `whole` are
+// one workgroup each, the streamed side of the `rest` is split over `parts`
+// workgroups.  Consecutive workgroups of an XCD take neighbouring tiles of a
+// head, which stream the same units.
+struct TileWork {
+    int tile, part, parts, slot;  // slot: place among the fp32 parts (-1: whole)
+};
+__device__ __forceinline__ TileWork tile_work(const BackwardTiles& p) {
+    if ((int)blockIdx.x < p.whole) return TileWork{xcd_remap(blockIdx.x, p.whole), 0, 1, -1};
+    const int item = xcd_remap(blockIdx.x - p.whole, p.rest * p.parts);
+    const int part = item / p.rest, t = item - part * p.rest;
+    return TileWork{p.whole + t, part, p.parts, p.parts > 1 ? item : -1};
+}
+
 // The gradient of one 32-column unit: to its rows, or, where the streamed side
 // is split over several workgroups, in fp32 to this part's slot (summed in order
 // by attention_backward_join_kernel).  Element (lane, v) of tile md of a slot is at
@@ -299,27 +355,33 @@ __device__ __forceinline__ void store_unit(const f32x16 (&g)[MD], float factor, 
     }
 }
 
-// Sums the parts of one tensor's units in order and stores the rows; one wave
-// per (head, unit, tile).
-template <typename T, int MD>
-__global__ __launch_bounds__(64) void attention_backward_join_kernel(const float* part, int parts, int64_t part_floats,
-                                                                     int units, int tokens, int d_real, OutView out) {
+// Sums the parts of the split tiles in order and stores their rows; one wave per
+// (tensor, tile, unit of the tile, 32 dims).
+template <typename T, int MD, int UNITS>
+__global__ __launch_bounds__(64) void attention_backward_join_kernel(const float* part, BackwardTiles p, int units, int tokens,
+                                                                     int d_real, OutView out0, OutView out1) {
     const int lane = threadIdx.x;
     const int md = blockIdx.x % MD;
-    const int work = blockIdx.x / MD;
-    const int bh = work / units;
-    const int unit = work - bh * units;
-    const float* src = part + ((int64_t)work * MD + md) * 1024 + lane * 4;
+    int work = blockIdx.x / MD;
+    const int u = work % UNITS;
+    work /= UNITS;
+    const int tensor = work / p.rest, t = work - tensor * p.rest;
+    const int bh = (p.whole + t) / p.per_head;
+    const int unit = ((p.whole + t) - bh * p.per_head) * UNITS + u;
+    if (unit >= units) return;
+    const int64_t slots = (int64_t)p.rest * UNITS * MD * 1024;  // floats of one part of one tensor
+    const float* src = part + tensor * p.parts * slots + (((int64_t)t * UNITS + u) * MD + md) * 1024 + lane * 4;
     f32x16 x;
 #pragma unroll
     for (int v = 0; v < 16; ++v) x[v] = 0.0f;
-    for (int i = 0; i < parts; ++i)
+    for (int i = 0; i < p.parts; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const f32x4 y = *reinterpret_cast<const f32x4*>(src + i * part_floats + q * 256);
+            const f32x4 y = *reinterpret_cast<const f32x4*>(src + i * slots + q * 256);
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[4 * q + e] += y[e];
         }
+    const OutView& out = tensor == 0 ? out0 : out1;
     const int token = unit * kUnit + (lane & 31);
     if (token < tokens)
         store_tile<T>(reinterpret_cast<T*>(out.data) + out.row(bh, token), md * 32, d_real, x, lane >> 5);
@@ -330,18 +392,15 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void attention_backward_kv_kernel(BackwardArgs a) {
     typedef typename Elem<T>::vec8 vec8;
-    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = q_unit_frags<D>(), S = stages<D>();
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = q_unit_frags<D>(), S = stages<D>(), R = 4;
     constexpr int kBytes = FRAGS * 1024;
-    constexpr int kCopies = (FRAGS + kWaves - 1) / kWaves;
     __shared__ __attribute__((aligned(1024))) char lds_buf[S * kBytes];
     lds_char* const lds = (lds_char*)lds_buf;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int tiles = (a.kv_units + kWaves * N - 1) / (kWaves * N);
-    const int work = xcd_remap(blockIdx.x, gridDim.x);
-    const int tile = work % tiles;
-    const int part = work / tiles % a.kv_parts;
-    const int bh = work / (tiles * a.kv_parts);
+    const TileWork work = tile_work(a.kv_tiles);
+    const int bh = work.tile / a.kv_tiles.per_head;
+    const int tile = work.tile - bh * a.kv_tiles.per_head;
     const int batch = bh / a.k.heads;
     const int length = a.length(batch);
     const int unit0 = (tile * kWaves + wave) * N;
@@ -350,7 +409,7 @@ void attention_backward_kv_kernel(BackwardArgs a) {
     // steps: the live query units of each of the group's heads, one after the other
     const int q_live = (a.q_tokens + kUnit - 1) / kUnit;
     const int steps = tile * kWaves * N * kUnit < length ? a.kv_group * q_live : 0;
-    const int i0 = (int)((int64_t)steps * part / a.kv_parts), i1 = (int)((int64_t)steps * (part + 1) / a.kv_parts);
+    const int i0 = (int)((int64_t)steps * work.part / work.parts), i1 = (int)((int64_t)steps * (work.part + 1) / work.parts);
     const char* const table = a.qx + (int64_t)bh * a.kv_group * a.q_units * kBytes;  // heads bh * group ..
     auto unit_of = [&](int i) {
         i = min(i, i1 - 1);
@@ -370,7 +429,10 @@ void attention_backward_kv_kernel(BackwardArgs a) {
     }
     const float f = __builtin_amdgcn_exp2f(e - kShift16);
 
-    vec8 kf[N][KT], vf[N][KT];
+    constexpr int NV = kValuesInLds<D> ? N - 1 : N;
+    __shared__ __attribute__((aligned(1024))) char own_buf[kValuesInLds<D> ? kWaves * KT * 1024 : 16];
+    lds_char* const own_v = (lds_char*)own_buf + (kValuesInLds<D> ? wave * KT * 1024 + lane * 16 : 0);
+    vec8 kf[N][KT], vf[NV][KT];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const char* own = a.kx + ((int64_t)bh * a.kv_units + min(unit0 + n, a.kv_units - 1)) * (kv_unit_frags<D>() * 1024) +
@@ -378,7 +440,11 @@ void attention_backward_kv_kernel(BackwardArgs a) {
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             kf[n][t] = load8<vec8>(own + t * 1024);
-            vf[n][t] = load8<vec8>(own + (KT + t) * 1024);
+            const vec8 x = load8<vec8>(own + (KT + t) * 1024);
+            if (n < NV)
+                vf[n][t] = x;
+            else
+                *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(own_v + t * 1024) = __builtin_bit_cast(u32x4, x);
         }
     }
     f32x16 dk[N][MD], dv[N][MD];
@@ -392,73 +458,88 @@ void attention_backward_kv_kernel(BackwardArgs a) {
     if (i0 < i1) {
         const uint32_t base = (uint32_t)(uintptr_t)lds;
         __builtin_amdgcn_s_waitcnt(kWaitVm0);  // the own operands: only copies are in flight from here on
+        copy_unit<FRAGS>(unit_of(i0), base, wave, lane * 16);
+        if constexpr (S == 3) copy_unit<FRAGS>(unit_of(i0 + 1), base + kBytes, wave, lane * 16);
+        wait_copies();
+        vec8 ring[R];  // the next fragments, read R steps ahead
 #pragma unroll
-        for (int s = 0; s < S - 1; ++s) copy_unit<FRAGS>(unit_of(i0 + s), base + s * kBytes, wave, lane);
-        stage_barrier<(S - 2) * kCopies>();
+        for (int j = 0; j < R; ++j) ring[j] = lds_frag<vec8>(lds + lane * 16 + j * 1024);
         int buf = 0;
         for (int i = i0; i < i1; ++i) {
-            copy_unit<FRAGS>(unit_of(i + S - 1), base + (buf == 0 ? S - 1 : buf - 1) * kBytes, wave, lane);
-            const lds_char* u = lds + buf * kBytes + lane * 16;
-            const lds_char* stat = lds + buf * kBytes + 4 * KT * 1024 + half * 16;
-            f32x16 s[N], dp[N], nl, nd;
+            const int next = buf == S - 1 ? 0 : buf + 1;
+            if constexpr (S == 2) copy_unit<FRAGS>(unit_of(i + 1), base + next * kBytes, wave, lane * 16);
+            const lds_char* const u = lds + buf * kBytes + lane * 16;
+            const lds_char* const un = lds + next * kBytes + lane * 16;
+            const lds_char* const stat = lds + buf * kBytes + 4 * KT * 1024 + half * 16;
+            pin_all(vf);
+            f32x16 s[N], dp[N], nl, nd, zero;
+            vec8 p[N][2], ds[N][2], vring[2];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 x = lds_frag<f32x4>(stat + q * 32), y = lds_frag<f32x4>(stat + 128 + q * 32);
+            for (int v = 0; v < 16; ++v) zero[v] = 0.0f;
+            unrolled<4 * KT>([&](auto index) __attribute__((always_inline)) {
+                constexpr int j = index, phase = j / KT, t = j % KT;
+                const vec8 x = ring[j % R];
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    nl[4 * q + z] = x[z];
-                    nd[4 * q + z] = y[z];
+                for (int n = 0; n < N; ++n) {
+                    if constexpr (phase == 0) s[n] = mfma32(x, kf[n][t], t == 0 ? zero : s[n]);
+                    if constexpr (phase == 1) dp[n] = mfma32(x, n < NV ? vf[n][t] : vring[t % 2], t == 0 ? nd : dp[n]);
+                    if constexpr (phase == 2) dv[n][t % MD] = mfma32(x, p[n][t / MD], dv[n][t % MD]);
+                    if constexpr (phase == 3) dk[n][t % MD] = mfma32(x, ds[n][t / MD], dk[n][t % MD]);
                 }
-            }
+                if constexpr (j + R < 4 * KT)
+                    ring[j % R] = lds_frag<vec8>(u + (j + R) * 1024);
+                else if constexpr (S == 3)
+                    ring[j % R] = lds_frag<vec8>(un + (j + R - 4 * KT) * 1024);
+                if constexpr (kValuesInLds<D> && ((phase == 0 && t >= KT - 2) || (phase == 1 && t < KT - 2)))
+                    vring[t % 2] = lds_frag<vec8>(own_v + (phase == 0 ? t - (KT - 2) : t + 2) * 1024);
+                if constexpr (phase == 0 && t >= KT - 4) {  // four rows of dL - delta
+                    constexpr int q = t - (KT - 4);
+                    const f32x4 y = lds_frag<f32x4>(stat + 128 + q * 32);
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s[n][v] = 0.0f;
-                dp[n] = nd;
-            }
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const vec8 x = lds_frag<vec8>(u + t * 1024);
-#pragma unroll
-                for (int n = 0; n < N; ++n) s[n] = mfma32(x, kf[n][t], s[n]);
-            }
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const vec8 x = lds_frag<vec8>(u + (KT + t) * 1024);
-#pragma unroll
-                for (int n = 0; n < N; ++n) dp[n] = mfma32(x, vf[n][t], dp[n]);
-            }
-            vec8 p[N][2];
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    s[n][v] = __builtin_amdgcn_exp2f(fmaf(s[n][v], c, nl[v]));
-                    p[n][v >> 3][v & 7] = from_f32<T>(s[n][v]);
+                    for (int w = 0; w < 4; ++w) nd[4 * q + w] = y[w];
                 }
+                if constexpr ((phase == 0 && t == KT - 1) || (phase == 1 && t == KT / 2 - 1)) {  // eight rows of -L
 #pragma unroll
-            for (int ss = 0; ss < 2; ++ss)
+                    for (int q = 2 * phase; q < 2 * phase + 2; ++q) {
+                        const f32x4 y = lds_frag<f32x4>(stat + q * 32);
 #pragma unroll
-                for (int md = 0; md < MD; ++md) {
-                    const vec8 x = lds_frag<vec8>(u + (3 * KT + md * 2 + ss) * 1024);
-#pragma unroll
-                    for (int n = 0; n < N; ++n) dv[n][md] = mfma32(x, p[n][ss], dv[n][md]);
+                        for (int w = 0; w < 4; ++w) nl[4 * q + w] = y[w];
+                    }
                 }
+                // probabilities beside the products of dP, dS beside those of dV: pairs of
+                // elements in the order (rows 0-15 of each tile, then rows 16-31), from the
+                // second step on (the first still waits for the last product)
+                if constexpr ((phase == 1 || phase == 2) && t > 0) {
+                    constexpr int from = (t - 1) * 8 * N / (KT - 1), to = t * 8 * N / (KT - 1);
+                    unrolled<to - from>([&](auto offset) __attribute__((always_inline)) {
+                        constexpr int y = from + offset, n = y / 4 % N, ss = y / (4 * N);
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    p[n][v >> 3][v & 7] = from_f32<T>(kScaled<T> ? s[n][v] * (dp[n][v] * f) : s[n][v] * dp[n][v]);
-#pragma unroll
-            for (int ss = 0; ss < 2; ++ss)
-#pragma unroll
-                for (int md = 0; md < MD; ++md) {
-                    const vec8 x = lds_frag<vec8>(u + (2 * KT + md * 2 + ss) * 1024);
-#pragma unroll
-                    for (int n = 0; n < N; ++n) dk[n][md] = mfma32(x, p[n][ss], dk[n][md]);
+                        for (int w = 0; w < 2; ++w) {
+                            const int e = 2 * (y % 4) + w, v = 8 * ss + e;
+                            if constexpr (phase == 1) {
+                                s[n][v] = __builtin_amdgcn_exp2f(fmaf(s[n][v], c, nl[v]));
+                                p[n][ss][e] = from_f32<T>(s[n][v]);
+                            } else {
+                                ds[n][ss][e] = from_f32<T>(kScaled<T> ? (s[n][v] * f) * dp[n][v] : s[n][v] * dp[n][v]);
+                            }
+                        }
+                    });
                 }
-            buf = buf == S - 1 ? 0 : buf + 1;
-            stage_barrier<(S - 2) * kCopies>();
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (S == 3 && j == 2 * KT - 1) {
+                    // every wave is past unit i - 1, and unit i + 1 has landed: its buffer is the
+                    // first one's to fill and the other may be read ahead
+                    wait_copies();
+                    copy_unit<FRAGS>(unit_of(i + 2), base + (buf == 0 ? S - 1 : buf - 1) * kBytes, wave, lane * 16);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            });
+            if constexpr (S == 2) {
+                wait_copies();
+#pragma unroll
+                for (int j = 0; j < R; ++j) ring[j] = lds_frag<vec8>(un + j * 1024);
+            }
+            buf = next;
         }
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // no copy outlives the workgroup's LDS
     }
@@ -471,10 +552,9 @@ void attention_backward_kv_kernel(BackwardArgs a) {
         const bool inside = key < a.kv_tokens, live = key < length;
         const int64_t at = inside ? key : 0;
         float* slot = nullptr;
-        if (a.kv_parts > 1)
-            slot = a.part + (((int64_t)part * 2 * a.batch * a.k.heads + bh) * a.kv_units + unit) * MD * 1024;
+        if (work.slot >= 0) slot = a.part + (((int64_t)work.slot * kWaves + wave) * N + n) * MD * 1024;
         store_unit<T, MD>(dk[n], kfac, live, slot, reinterpret_cast<T*>(a.dk.data) + a.dk.row(bh, at), inside, a.head_dim, lane);
-        if (slot) slot += (int64_t)a.batch * a.k.heads * a.kv_units * MD * 1024;
+        if (slot) slot += (int64_t)a.kv_tiles.parts * a.kv_tiles.rest * kWaves * N * MD * 1024;
         store_unit<T, MD>(dv[n], vfac, live, slot, reinterpret_cast<T*>(a.dv.data) + a.dv.row(bh, at), inside, a.head_dim, lane);
     }
 }
@@ -484,26 +564,25 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void attention_backward_q_kernel(BackwardArgs a) {
     typedef typename Elem<T>::vec8 vec8;
-    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kv_unit_frags<D>(), S = stages<D>();
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kv_unit_frags<D>(), S = 3, R = 6;
     constexpr int kBytes = FRAGS * 1024;
-    constexpr int kCopies = (FRAGS + kWaves - 1) / kWaves;
     __shared__ __attribute__((aligned(1024))) char lds_buf[S * kBytes];
     lds_char* const lds = (lds_char*)lds_buf;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int tiles = (a.q_units + kWaves * N - 1) / (kWaves * N);
-    const int work = xcd_remap(blockIdx.x, gridDim.x);
-    const int tile = work % tiles;
-    const int part = work / tiles % a.q_parts;
-    const int bh = work / (tiles * a.q_parts);
+    const TileWork work = tile_work(a.q_tiles);
+    const int bh = work.tile / a.q_tiles.per_head;
+    const int tile = work.tile - bh * a.q_tiles.per_head;
     const int kv_bh = bh / a.kv_group;
     const int length = a.length(bh / a.heads);
     const int unit0 = (tile * kWaves + wave) * N;
     const float c = a.scale_log2;
     const int steps = (length + kUnit - 1) / kUnit;
-    const int i0 = (int)((int64_t)steps * part / a.q_parts), i1 = (int)((int64_t)steps * (part + 1) / a.q_parts);
+    const int i0 = (int)((int64_t)steps * work.part / work.parts), i1 = (int)((int64_t)steps * (work.part + 1) / work.parts);
     const char* const table = a.kx + (int64_t)kv_bh * a.kv_units * kBytes;
     auto unit_of = [&](int i) { return table + (int64_t)min(i, i1 - 1) * kBytes; };
+    // fragment of the buffer used j-th: K rows, K^T, V rows
+    auto order = [](int j) { return j < KT ? j : j < 2 * KT ? j + KT : j - KT; };
 
     float e = 0.0f;
     if constexpr (kScaled<T>) {
@@ -538,61 +617,91 @@ void attention_backward_q_kernel(BackwardArgs a) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) dq[n][md][v] = 0.0f;
 
+    // Step i forms S and dP of unit i and adds unit i - 1 to dQ: dS of i - 1 is formed
+    // beside the products of S, the probabilities of i beside those of dQ.  The
+    // buffer of step i therefore holds K and V rows of unit i and K^T of i - 1.
     if (i0 < i1) {
         const uint32_t base = (uint32_t)(uintptr_t)lds;
+        auto copy_step = [&](int i, int b) {
+            copy_unit<FRAGS, 2 * KT>(unit_of(i), unit_of(max(i - 1, i0)), base + b * kBytes, wave, lane * 16);
+        };
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
+        copy_step(i0, 0);
+        copy_step(i0 + 1, 1);
+        wait_copies();
+        vec8 ring[R];
 #pragma unroll
-        for (int s = 0; s < S - 1; ++s) copy_unit<FRAGS>(unit_of(i0 + s), base + s * kBytes, wave, lane);
-        stage_barrier<(S - 2) * kCopies>();
+        for (int j = 0; j < R; ++j) ring[j] = lds_frag<vec8>(lds + lane * 16 + order(j) * 1024);
+        f32x16 s[N], dp[N];
         int buf = 0;
-        for (int i = i0; i < i1; ++i) {
-            copy_unit<FRAGS>(unit_of(i + S - 1), base + (buf == 0 ? S - 1 : buf - 1) * kBytes, wave, lane);
-            const lds_char* u = lds + buf * kBytes + lane * 16;
-            f32x16 s[N], dp[N];
+        // first: there is no unit i - 1; last: no unit i
+        auto step = [&](int i, auto is_first, auto is_last) __attribute__((always_inline)) {
+            constexpr bool first = is_first, last = is_last;
+            const int next = buf == S - 1 ? 0 : buf + 1;
+            const lds_char* const u = lds + buf * kBytes + lane * 16;
+            const lds_char* const un = lds + next * kBytes + lane * 16;
+            pin_all(qf);
+            pin_all(of);
+            f32x16 sn[N], zero, start[N];
+            vec8 ds[N][2];
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+            for (int v = 0; v < 16; ++v) {
+                zero[v] = 0.0f;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    s[n][v] = 0.0f;
-                    dp[n][v] = nd[n];
+                for (int n = 0; n < N; ++n) start[n][v] = nd[n];
+            }
+            unrolled<3 * KT>([&](auto index) __attribute__((always_inline)) {
+                constexpr int j = index, phase = j / KT, t = j % KT;
+                const vec8 x = ring[j % R];
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    if constexpr (phase == 0 && !last) sn[n] = mfma32(x, qf[n][t], t == 0 ? zero : sn[n]);
+                    if constexpr (phase == 1 && !first) dq[n][t % MD] = mfma32(x, ds[n][t / MD], dq[n][t % MD]);
+                    if constexpr (phase == 2 && !last) dp[n] = mfma32(x, of[n][t], t == 0 ? start[n] : dp[n]);
                 }
+                if constexpr (j + R < 3 * KT)
+                    ring[j % R] = lds_frag<vec8>(u + order(j + R) * 1024);
+                else if constexpr (!last)
+                    ring[j % R] = lds_frag<vec8>(un + order(j + R - 3 * KT) * 1024);
+                if constexpr (phase == 0 ? !first : phase == 1 && !last && t > 0) {
+                    constexpr int part = phase == 0 ? t : t - 1, parts = phase == 0 ? KT : KT - 1;
+                    constexpr int from = part * 8 * N / parts, to = (part + 1) * 8 * N / parts;
+                    unrolled<to - from>([&](auto offset) __attribute__((always_inline)) {
+                        constexpr int y = from + offset, n = y / 4 % N, ss = y / (4 * N);
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const vec8 x = lds_frag<vec8>(u + t * 1024);
-#pragma unroll
-                for (int n = 0; n < N; ++n) s[n] = mfma32(x, qf[n][t], s[n]);
-            }
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const vec8 x = lds_frag<vec8>(u + (KT + t) * 1024);
-#pragma unroll
-                for (int n = 0; n < N; ++n) dp[n] = mfma32(x, of[n][t], dp[n]);
-            }
-            if ((i + 1) * kUnit > length) {  // the last unit's masked keys: probability 0
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (i * kUnit + 8 * (v >> 2) + 4 * half + (v & 3) >= length)
-#pragma unroll
-                        for (int n = 0; n < N; ++n) s[n][v] = -__builtin_inff();
-            }
-            vec8 p[N][2];
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    p[n][v >> 3][v & 7] = from_f32<T>(__builtin_amdgcn_exp2f(fmaf(s[n][v], c, nl[n])) * dp[n][v]);
-#pragma unroll
-            for (int ss = 0; ss < 2; ++ss)
-#pragma unroll
-                for (int md = 0; md < MD; ++md) {
-                    const vec8 x = lds_frag<vec8>(u + (2 * KT + md * 2 + ss) * 1024);
-#pragma unroll
-                    for (int n = 0; n < N; ++n) dq[n][md] = mfma32(x, p[n][ss], dq[n][md]);
+                        for (int w = 0; w < 2; ++w) {
+                            const int e = 2 * (y % 4) + w, v = 8 * ss + e;
+                            if constexpr (phase == 0)
+                                ds[n][ss][e] = from_f32<T>(s[n][v] * dp[n][v]);
+                            else
+                                sn[n][v] = __builtin_amdgcn_exp2f(fmaf(sn[n][v], c, nl[n]));
+                        }
+                    });
                 }
-            buf = buf == S - 1 ? 0 : buf + 1;
-            stage_barrier<(S - 2) * kCopies>();
-        }
-        __builtin_amdgcn_s_waitcnt(kWaitVm0);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (j == KT - 1) {
+                    if (!last && (i + 1) * kUnit > length) {  // the last unit's masked keys: probability 0
+                        asm volatile("");  // a branch, not selects in every step
+#pragma unroll
+                        for (int v = 0; v < 16; ++v)
+                            if (i * kUnit + 8 * (v >> 2) + 4 * half + (v & 3) >= length)
+#pragma unroll
+                                for (int n = 0; n < N; ++n) sn[n][v] = -__builtin_inff();
+                    }
+                    // every wave is past step i - 1, and step i + 1's fragments have landed
+                    wait_copies();
+                    if constexpr (!last) copy_step(i + 2, buf == 0 ? S - 1 : buf - 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            });
+#pragma unroll
+            for (int n = 0; n < N; ++n) s[n] = sn[n];
+            buf = next;
+        };
+        step(i0, std::true_type{}, std::false_type{});
+        for (int i = i0 + 1; i < i1; ++i) step(i, std::false_type{}, std::false_type{});
+        step(i1, std::false_type{}, std::true_type{});
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     }
     const float fac = a.scale * __builtin_amdgcn_exp2f(-e);
 #pragma unroll
@@ -602,7 +711,7 @@ void attention_backward_q_kernel(BackwardArgs a) {
         const int row = unit * kUnit + col;
         const bool inside = row < a.q_tokens;
         float* slot = nullptr;
-        if (a.q_parts > 1) slot = a.part + (((int64_t)part * a.batch * a.heads + bh) * a.q_units + unit) * MD * 1024;
+        if (work.slot >= 0) slot = a.part + (((int64_t)work.slot * kWaves + wave) * N + n) * MD * 1024;
         store_unit<T, MD>(dq[n], fac, true, slot, reinterpret_cast<T*>(a.dq.data) + a.dq.row(bh, inside ? row : 0), inside,
                           a.head_dim, lane);
     }
@@ -616,30 +725,23 @@ int launch_t(const BackwardArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((attention_backward_pack_kernel<T, D>), dim3(bh * (a.q_units / 2) + kv_bh * (a.kv_units / 2)), dim3(256),
                        0, stream, a);
     if ((rc = pisa_host::check_launch("attention_backward_pack_kernel"))) return rc;
+    auto workgroups = [](const BackwardTiles& p) { return dim3(p.whole + p.rest * p.parts); };
+    auto join = [&](const BackwardTiles& p, int tensors, int units, int tokens, const OutView& out0, const OutView& out1) {
+        if (p.parts <= 1) return PISA_OK;
+        hipLaunchKernelGGL((attention_backward_join_kernel<T, MD, kTile>), dim3(tensors * p.rest * kTile * MD), dim3(64), 0,
+                           stream, a.part, p, units, tokens, a.head_dim, out0, out1);
+        return pisa_host::check_launch("attention_backward_join_kernel");
+    };
     if (a.dk.data) {
-        hipLaunchKernelGGL((attention_backward_kv_kernel<T, D>), dim3(kv_bh * a.kv_parts * ((a.kv_units + kTile - 1) / kTile)),
-                           dim3(64 * kWaves), 0, stream, a);
-        if ((rc = pisa_host::check_launch("attention_backward_kv_kernel"))) return rc;
-        if (a.kv_parts > 1) {
-            const int64_t tensor = (int64_t)kv_bh * a.kv_units * MD * 1024;
-            for (int i = 0; i < 2; ++i) {
-                hipLaunchKernelGGL((attention_backward_join_kernel<T, MD>), dim3(kv_bh * a.kv_units * MD), dim3(64), 0, stream,
-                                   a.part + i * tensor, a.kv_parts, 2 * tensor, a.kv_units, a.kv_tokens, a.head_dim,
-                                   i == 0 ? a.dk : a.dv);
-                if ((rc = pisa_host::check_launch("attention_backward_join_kernel"))) return rc;
-            }
-        }
+        hipLaunchKernelGGL((attention_backward_kv_kernel<T, D>), workgroups(a.kv_tiles), dim3(64 * kWaves), 0, stream, a);
+        if ((rc = pisa_host::check_launch("attention_backward_kv_kernel")) ||
+            (rc = join(a.kv_tiles, 2, a.kv_units, a.kv_tokens, a.dk, a.dv)))
+            return rc;
     }
     if (!a.dq.data) return PISA_OK;
-    hipLaunchKernelGGL((attention_backward_q_kernel<T, D>), dim3(bh * a.q_parts * ((a.q_units + kTile - 1) / kTile)),
-                       dim3(64 * kWaves), 0, stream, a);
+    hipLaunchKernelGGL((attention_backward_q_kernel<T, D>), workgroups(a.q_tiles), dim3(64 * kWaves), 0, stream, a);
     if ((rc = pisa_host::check_launch("attention_backward_q_kernel"))) return rc;
-    if (a.q_parts > 1) {
-        hipLaunchKernelGGL((attention_backward_join_kernel<T, MD>), dim3(bh * a.q_units * MD), dim3(64), 0, stream, a.part,
-                           a.q_parts, (int64_t)bh * a.q_units * MD * 1024, a.q_units, a.q_tokens, a.head_dim, a.dq);
-        rc = pisa_host::check_launch("attention_backward_join_kernel");
-    }
-    return rc;
+    return join(a.q_tiles, 1, a.q_units, a.q_tokens, a.dq, a.dq);
 }
 
 template <typename T>
@@ -657,32 +759,38 @@ int launch_d(int padded, const BackwardArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// How many workgroups share the streamed side of one tile of columns: as many
-// as the 256 CUs hold beside each other, while each part keeps eight units.
-static int parts_for(int64_t workgroups, int64_t steps) {
-    constexpr int64_t kSlots = 256;
-    int64_t n = workgroups > 0 ? kSlots / workgroups : 1;
-    if (n > steps / 8) n = steps / 8;
-    return n < 1 ? 1 : static_cast<int>(n);
+// A tile's workgroup has a CU to itself, so the tiles run in rounds of 256.  Those
+// of the last, partial round (all of them in a small problem) are split over as
+// many workgroups as fill the CUs, while each part keeps eight units.
+static BackwardTiles split_tiles(int64_t heads, int units, int units_per_tile, int64_t steps) {
+    constexpr int kSlots = 256;
+    BackwardTiles p;
+    p.per_head = (units + units_per_tile - 1) / units_per_tile;
+    const int64_t tiles = heads * p.per_head;
+    p.whole = static_cast<int>(tiles / kSlots * kSlots);
+    p.rest = static_cast<int>(tiles - p.whole);
+    int64_t parts = p.rest > 0 ? kSlots / p.rest : 1;
+    if (parts > steps / 8) parts = steps / 8;
+    p.parts = parts < 1 ? 1 : static_cast<int>(parts);
+    return p;
 }
 
 BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int padded, bool scaled) {
     BackwardPlan p;
-    const int columns_per_tile = kWaves * (padded <= 128 ? 2 : 1);
+    const int tile = kWaves * (padded <= 128 ? 2 : 1);
     p.q_units = (q_tokens + kBlock - 1) / kBlock * 2;
     p.kv_units = (kv_tokens + kBlock - 1) / kBlock * 2;
     const int64_t bh = (int64_t)batch * heads, kv_bh = (int64_t)batch * kv_heads;
-    p.q_parts = parts_for(bh * ((p.q_units + columns_per_tile - 1) / columns_per_tile), p.kv_units);
-    p.kv_parts = parts_for(kv_bh * ((p.kv_units + columns_per_tile - 1) / columns_per_tile),
-                           (int64_t)p.q_units * (heads / kv_heads));
+    p.q_tiles = split_tiles(bh, p.q_units, tile, p.kv_units);
+    p.kv_tiles = split_tiles(kv_bh, p.kv_units, tile, (int64_t)p.q_units * (heads / kv_heads));
     p.qx_bytes = bh * p.q_units * (4 * (padded / 16) + 1) * 1024;
     p.kx_bytes = kv_bh * p.kv_units * 3 * (padded / 16) * 1024;
     p.q_most_bytes = scaled ? bh * (p.q_units / 2) * (int64_t)sizeof(float) : 0;
     p.l_most_bytes = p.q_most_bytes;
     p.v_most_bytes = scaled ? kv_bh * (p.kv_units / 2) * (int64_t)sizeof(float) : 0;
-    const int64_t tile_bytes = (int64_t)padded * kUnit * sizeof(float);
-    const int64_t q_part = p.q_parts > 1 ? p.q_parts * bh * p.q_units * tile_bytes : 0;
-    const int64_t kv_part = p.kv_parts > 1 ? 2 * p.kv_parts * kv_bh * p.kv_units * tile_bytes : 0;
+    const int64_t tile_bytes = (int64_t)tile * padded * kUnit * sizeof(float);
+    const int64_t q_part = p.q_tiles.parts > 1 ? p.q_tiles.parts * p.q_tiles.rest * tile_bytes : 0;
+    const int64_t kv_part = p.kv_tiles.parts > 1 ? 2 * p.kv_tiles.parts * p.kv_tiles.rest * tile_bytes : 0;
     p.part_bytes = q_part > kv_part ? q_part : kv_part;  // the two kernels run one after the other
     return p;
 }

@@ -292,6 +292,9 @@ int norm_rope_parts(const NormRopeArgs& g);
 int launch_norm_rope(int dtype, const NormRopeArgs& g, bool backward, hipStream_t stream);
 
 // Backward pass of dense attention (attention_backward.hip).
+struct BackwardTiles {
+    int per_head, whole, rest, parts;  // tiles of a head; tiles run whole, tiles split, workgroups of a split one
+};
 struct BackwardArgs {
     View q, k, v, o, dout;
     OutView dq, dk, dv;         // dq, or dk and dv, may be null: not formed
@@ -300,8 +303,9 @@ struct BackwardArgs {
     const int32_t* kv_lengths;  // [B] or null
     int batch, heads, kv_group, q_tokens, kv_tokens, head_dim;
     float scale, scale_log2;
-    // plan_backward: 32-row units (an even number) and the parts of the streamed side
-    int q_units, kv_units, q_parts, kv_parts;
+    // plan_backward: 32-row units (an even number) and the tiles of the launches
+    int q_units, kv_units;
+    BackwardTiles q_tiles, kv_tiles;
     char *qx, *kx;              // packed units
     // largest row norms of dO and V and largest |dlse| by 64-row block (fp16): [BH][q_units/2], [BHk][kv_units/2]
     float *q_most, *v_most, *l_most;
@@ -311,7 +315,8 @@ struct BackwardArgs {
     }
 };
 struct BackwardPlan {
-    int q_units, kv_units, q_parts, kv_parts;
+    int q_units, kv_units;
+    BackwardTiles q_tiles, kv_tiles;
     int64_t qx_bytes, kx_bytes, q_most_bytes, v_most_bytes, l_most_bytes, part_bytes;
 };
 BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int padded, bool scaled);
