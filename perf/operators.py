@@ -260,9 +260,8 @@ def _plain_train(s):
 
 # ------------------------------------------------------------------ one pass
 def _package():
-    path = str(pathlib.Path(__file__).resolve().parents[1] / "comfyui-rdna35-attention_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
+    if "mi355x_pisa" not in sys.modules:
+        sys.path.insert(0, str(pathlib.Path(__file__).resolve().parents[1] / "comfyui-rdna35-attention_amd"))
     import mi355x_pisa
 
     return mi355x_pisa
