@@ -1036,8 +1036,14 @@ static int fill_norm_rope(const char* what, int dtype, int weight_dtype, int bat
     a.head_dim = head_dim;
     a.eps = eps;
     a.weight_f32 = weight_dtype == PISA_DTYPE_F32;
-    pisa::norm_rope_split(a);
     return PISA_OK;
+}
+
+static int split_norm_rope(const char* what, pisa::NormRopeArgs& a) {
+    pisa::norm_rope_split(a);
+    if (a.tiles <= kMaxGridBlocks) return PISA_OK;
+    return fail(PISA_ERR_UNSUPPORTED, "%s supports %lld tiles of %d tokens, got B=%d T=%d", what, (long long)kMaxGridBlocks,
+                a.tile_tokens, a.batch, a.tokens);
 }
 
 // Base pointer aligned to the element (the kernels need no more).
@@ -1070,6 +1076,7 @@ int attn_hip_qk_norm_rope(int32_t dtype, int32_t weight_dtype, int32_t batch, in
         a.out[1] = to_out(k_out, k_heads);
         a.weight[1] = k_weight;
     }
+    if ((rc = split_norm_rope("qk_norm_rope", a))) return rc;
     return pisa::launch_norm_rope(dtype, a, false, static_cast<hipStream_t>(stream));
 }
 
@@ -1115,6 +1122,7 @@ int attn_hip_qk_norm_rope_backward(int32_t dtype, int32_t weight_dtype, int32_t 
         a.weight_grad[1] = dk_weight;
     }
     a.partial = weights ? static_cast<float*>(workspace) : nullptr;
+    if ((rc = split_norm_rope("qk_norm_rope_backward", a))) return rc;
     return pisa::launch_norm_rope(dtype, a, true, static_cast<hipStream_t>(stream));
 }
 

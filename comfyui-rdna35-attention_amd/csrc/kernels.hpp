@@ -282,8 +282,10 @@ struct NormRopeArgs {
     int heads[2], batch, tokens, head_dim;
     RopeArgs rope;
     // set by norm_rope_split
-    int rows_per_group, groups_per_token;
-    int64_t groups;
+    int tile_tokens, tile_shift, tiles_per_batch;
+    int64_t tiles;
+    int heads_first[2];      // rows of a tile: the heads of a token beside each other, else the tokens of a head
+    uint32_t inv_heads[2];
 };
 constexpr int kNormRopeParts = 1024;
 int norm_rope_lanes(int head_dim);

@@ -12,11 +12,16 @@
 // Each kernel reads a row once and writes it once, so HBM bounds it.  A row is
 // held by LP = 8, 16 or 32 lanes of 8 dims (4 pairs) each: one 16-byte load and
 // store per lane and row of a two-byte type when interleaved, two of 8 bytes
-// otherwise, and no exchange between lanes other than the norm's sums.  A group of LP lanes takes
-// `rows_per_group` heads of one token, so the cosines and sines of a lane's
-// four pairs are formed once for all of them and no table is read.  The angle in
-// turns is formed in fp64 (position * inv_freq loses its fraction in fp32 from a
-// few thousand turns on), its fraction is rounded to fp32.
+// otherwise, and no exchange between lanes other than the norm's sums.  A
+// workgroup takes all heads of a tile of tokens, neighbouring rows in memory
+// beside each other (the heads of a token where those are closer together than
+// its neighbours, else the tokens of a head), so that what it reads at a time is
+// one run of memory.  The cosines and sines of the tile's tokens are formed once,
+// into LDS, while its first rows are on their way, and no table is read.  The
+// angle in turns is formed in fp64 (position * inv_freq loses its fraction in
+// fp32 from a few thousand turns on), its fraction is rounded to fp32.
+#include <stdlib.h>
+
 #include "kernels.hpp"
 
 namespace pisa {
@@ -25,6 +30,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;  // rows in flight per lane
+constexpr int kTileTokens = 16;  // most tokens of a tile
+constexpr int kMostPairs = 128;
 
 // Vectors of N elements at any element alignment (global loads and stores
 // need no more on gfx950).
@@ -108,21 +115,35 @@ __device__ __forceinline__ double axis_position(const RopeArgs& r, int b, int t,
     return static_cast<const float*>(r.pos)[o];
 }
 
-// Cosine and sine of the lane's four pairs at token (b, t).
-__device__ __forceinline__ void lane_angles(const RopeArgs& r, int b, int t, int lane, float (&c)[4], float (&s)[4]) {
+// Cosines and sines of the tile's tokens, token j's pair p at [j * kMostPairs + p].
+struct Angles {
+    float c[kTileTokens * kMostPairs], s[kTileTokens * kMostPairs];
+};
+__device__ __forceinline__ void tile_angles(const RopeArgs& r, int b, int t0, int tokens, Angles& out) {
     constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
+    for (int i = threadIdx.x; i < tokens * r.pairs; i += kThreads) {
+        const int j = i / r.pairs;
+        const int p = i - j * r.pairs;
+        const int axis = (p >= r.axis_end[0]) + (p >= r.axis_end[1]) + (p >= r.axis_end[2]);
+        double turns = axis_position(r, b, t0 + j, axis) * r.inv_freq[p] * kTurn;
+        turns -= __builtin_rint(turns);
+        float s, c;
+        sincospif(2.0f * static_cast<float>(turns), &s, &c);
+        out.c[j * kMostPairs + p] = c;
+        out.s[j * kMostPairs + p] = r.inverse ? -s : s;
+    }
+}
+// Those of a lane's four pairs (one and zero past the rotated dims).
+__device__ __forceinline__ void lane_angles(const Angles& a, int j, int lane, bool turned, float (&c)[4], float (&s)[4]) {
+    f32x4 x = {1.0f, 1.0f, 1.0f, 1.0f}, y = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (turned) {
+        x = *reinterpret_cast<const f32x4*>(&a.c[j * kMostPairs + 4 * lane]);
+        y = *reinterpret_cast<const f32x4*>(&a.s[j * kMostPairs + 4 * lane]);
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int p = 4 * lane + e;
-        c[e] = 1.0f;
-        s[e] = 0.0f;
-        if (p < r.pairs) {
-            const int axis = (p >= r.axis_end[0]) + (p >= r.axis_end[1]) + (p >= r.axis_end[2]);
-            double turns = axis_position(r, b, t, axis) * r.inv_freq[p] * kTurn;
-            turns -= __builtin_rint(turns);
-            sincospif(2.0f * static_cast<float>(turns), &s[e], &c[e]);
-            if (r.inverse) s[e] = -s[e];
-        }
+        c[e] = x[e];
+        s[e] = y[e];
     }
 }
 
@@ -132,72 +153,98 @@ template <int LP> __device__ __forceinline__ float group_sum(float x) {
     return x;
 }
 
-// A group's token and its heads [h0, h1) of tensor i (0: queries, 1: keys).
-struct GroupWork {
-    int b, t, row0, row1;
+// A workgroup's tile: tokens t0 .. t0 + tokens - 1 of batch entry b.
+struct Tile {
+    int b, t0, tokens;
 };
-__device__ __forceinline__ GroupWork group_work(const NormRopeArgs& g, int64_t group) {
-    const int64_t token = group / g.groups_per_token;
-    const int part = static_cast<int>(group - token * g.groups_per_token);
-    GroupWork w;
-    w.b = static_cast<int>(token / g.tokens);
-    w.t = static_cast<int>(token - (int64_t)w.b * g.tokens);
-    w.row0 = part * g.rows_per_group;
-    w.row1 = min(w.row0 + g.rows_per_group, g.heads[0] + g.heads[1]);
+__device__ __forceinline__ Tile tile_of(const NormRopeArgs& g, int64_t tile) {
+    Tile w;
+    w.b = static_cast<int>(tile / g.tiles_per_batch);
+    w.t0 = static_cast<int>(tile - (int64_t)w.b * g.tiles_per_batch) * g.tile_tokens;
+    w.tokens = min(g.tile_tokens, g.tokens - w.t0);
     return w;
+}
+// Row r of a tensor's rows in the tile: its token (of the tile) and head.
+struct Row {
+    int j, h;
+};
+__device__ __forceinline__ int tile_rows(const NormRopeArgs& g, const Tile& w, int i) {
+    return (g.heads_first[i] ? w.tokens : g.tile_tokens) * g.heads[i];
+}
+__device__ __forceinline__ Row row_of(const NormRopeArgs& g, int i, int r) {
+    if (g.heads_first[i]) {  // g.inv_heads = ceil(2^32 / heads): exact for the few tokens of a tile
+        const int j = g.tile_tokens == 1 ? 0 : static_cast<int>(__umulhi(r, g.inv_heads[i]));
+        return Row{j, r - j * g.heads[i]};
+    }
+    return Row{r & (g.tile_tokens - 1), r >> g.tile_shift};
+}
+template <typename T> __device__ __forceinline__ const T* row_at(const View& v, const Tile& w, Row x) {
+    return reinterpret_cast<const T*>(v.data) + w.b * v.sb + x.h * v.sh + (w.t0 + x.j) * v.st;
+}
+template <typename T> __device__ __forceinline__ T* row_at(const OutView& v, const Tile& w, Row x) {
+    return reinterpret_cast<T*>(v.data) + w.b * v.sb + x.h * v.sh + (w.t0 + x.j) * v.st;
 }
 
 template <typename T, int LP, bool IL>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs g) {
+    constexpr int kSlots = kThreads / LP;
+    __shared__ __attribute__((aligned(16))) Angles angles;
     const int lane = threadIdx.x % LP;
+    const int slot = threadIdx.x / LP;
     const bool live = 8 * lane < g.head_dim;
+    const bool turned = 4 * lane < g.rope.pairs;
     const LaneDims d = live ? lane_dims<IL>(lane, g.rope.pairs) : LaneDims{0, 0};
     const float inv_d = 1.0f / static_cast<float>(g.head_dim);
-    // whole groups enter and leave the loop: no lane of a group's sums is missing
-    for (int64_t group = (int64_t)blockIdx.x * (kThreads / LP) + threadIdx.x / LP; group < g.groups;
-         group += (int64_t)gridDim.x * (kThreads / LP)) {
-        const GroupWork w = group_work(g, group);
-        float c[4], s[4];
-        lane_angles(g.rope, w.b, w.t, lane, c, s);
+    const Tile w = tile_of(g, blockIdx.x);
+    float a[kUnroll][4], b[kUnroll][4];
+    Row x[kUnroll];
+    // rows r, r + kSlots, ... of tensor i (past the last one, or on tokens past the tile's, a row that is there)
+    auto load = [&](int i, int r) __attribute__((always_inline)) {
+        const int rows = tile_rows(g, w, i);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int h0 = i == 0 ? w.row0 : max(w.row0 - g.heads[0], 0);
-            const int h1 = i == 0 ? min(w.row1, g.heads[0]) : w.row1 - g.heads[0];
-            if (h0 >= h1) continue;
-            float wa[4], wb[4];
-            load_weight<T, IL>(g, g.weight[i], live, d, wa, wb);
-            const T* src = reinterpret_cast<const T*>(g.in[i].data) + w.b * g.in[i].sb + w.t * g.in[i].st;
-            T* dst = reinterpret_cast<T*>(g.out[i].data) + w.b * g.out[i].sb + w.t * g.out[i].st;
-            for (int h = h0; h < h1; h += kUnroll) {
-                float a[kUnroll][4], b[kUnroll][4];
+        for (int u = 0; u < kUnroll; ++u) {
+            x[u] = row_of(g, i, min(r + u * kSlots, rows - 1));
+            load_row<T, IL>(row_at<T>(g.in[i], w, Row{min(x[u].j, w.tokens - 1), x[u].h}), d, a[u], b[u]);
+        }
+    };
+    load(0, slot);  // on its way while the angles are formed
+    if (g.rope.pairs) {
+        tile_angles(g.rope, w.b, w.t0, w.tokens, angles);
+        __syncthreads();
+    }
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u)  // rows past the last re-read it
-                    load_row<T, IL>(src + min(h + u, h1 - 1) * g.in[i].sh, d, a[u], b[u]);
+    for (int i = 0; i < 2; ++i) {
+        if (g.heads[i] == 0) continue;
+        const int rows = tile_rows(g, w, i);
+        float wa[4], wb[4];
+        load_weight<T, IL>(g, g.weight[i], live, d, wa, wb);
+        for (int r = slot; r < rows; r += kSlots * kUnroll) {
+            if (i == 1 || r != slot) load(i, r);
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-                    float r = 1.0f;
-                    if (g.norm) {
-                        float sq = 0.0f;
+            for (int u = 0; u < kUnroll; ++u) {
+                float n = 1.0f;
+                if (g.norm) {
+                    float sq = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sq = fmaf(a[u][e], a[u][e], fmaf(b[u][e], b[u][e], sq));
-                        r = 1.0f / sqrtf(fmaf(group_sum<LP>(live ? sq : 0.0f), inv_d, g.eps));
-                    }
-                    if (!live || h + u >= h1) continue;
-                    float x[4], y[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float p = a[u][e] * r * wa[e], q = b[u][e] * r * wb[e];
-                        x[e] = p * c[e] - q * s[e];
-                        y[e] = p * s[e] + q * c[e];
-                    }
-                    store_row<T, IL>(dst + (h + u) * g.out[i].sh, d, x, y);
+                    for (int e = 0; e < 4; ++e) sq = fmaf(a[u][e], a[u][e], fmaf(b[u][e], b[u][e], sq));
+                    n = rsqrtf(fmaf(group_sum<LP>(live ? sq : 0.0f), inv_d, g.eps));
                 }
+                if (!live || r + u * kSlots >= rows || x[u].j >= w.tokens) continue;
+                float c[4], s[4], y[4], z[4];
+                lane_angles(angles, x[u].j, lane, turned, c, s);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = a[u][e] * n * wa[e], q = b[u][e] * n * wb[e];
+                    y[e] = p * c[e] - q * s[e];
+                    z[e] = p * s[e] + q * c[e];
+                }
+                store_row<T, IL>(row_at<T>(g.out[i], w, x[u]), d, y, z);
             }
         }
     }
 }
 
-// The backward pass.  Workgroups walk the groups with the grid's stride and keep
+// The backward pass.  Workgroups walk the tiles with the grid's stride and keep
 // the weight gradients of their rows in registers; the row slots of a workgroup
 // are added through LDS in order and written as one partial per workgroup
 // (partial[tensor][dim][workgroup]), which norm_rope_weights_kernel sums: the
@@ -205,64 +252,68 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs g) {
 template <typename T, int LP, bool IL>
 __global__ __launch_bounds__(kThreads) void norm_rope_backward_kernel(NormRopeArgs g) {
     constexpr int kSlots = kThreads / LP;
-    constexpr int kRows = 2;  // two tensors to read: as many loads in flight as the forward kernel
+    constexpr int kRows = 1;  // more in flight bring nothing here, and cost waves
+    __shared__ __attribute__((aligned(16))) Angles angles;
     __shared__ float lds[kSlots][LP * 8];
     const int lane = threadIdx.x % LP;
     const int slot = threadIdx.x / LP;
     const bool live = 8 * lane < g.head_dim;
+    const bool turned = 4 * lane < g.rope.pairs;
     const LaneDims d = live ? lane_dims<IL>(lane, g.rope.pairs) : LaneDims{0, 0};
     const float inv_d = 1.0f / static_cast<float>(g.head_dim);
-    float da[2][4], db[2][4];
+    float da[2][4], db[2][4], wa[2][4], wb[2][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+        load_weight<T, IL>(g, g.weight[i], live, d, wa[i], wb[i]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) da[i][e] = db[i][e] = 0.0f;
-    for (int64_t group = (int64_t)blockIdx.x * kSlots + slot; group < g.groups; group += (int64_t)gridDim.x * kSlots) {
-        const GroupWork w = group_work(g, group);
-        float c[4], s[4];
-        lane_angles(g.rope, w.b, w.t, lane, c, s);
+    }
+    for (int64_t tile = blockIdx.x; tile < g.tiles; tile += gridDim.x) {
+        const Tile w = tile_of(g, tile);
+        if (g.rope.pairs) {
+            if (tile != blockIdx.x) __syncthreads();  // the last tile's angles are read
+            tile_angles(g.rope, w.b, w.t0, w.tokens, angles);
+            __syncthreads();
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int h0 = i == 0 ? w.row0 : max(w.row0 - g.heads[0], 0);
-            const int h1 = i == 0 ? min(w.row1, g.heads[0]) : w.row1 - g.heads[0];
-            if (h0 >= h1) continue;
-            float wa[4], wb[4];
-            load_weight<T, IL>(g, g.weight[i], live, d, wa, wb);
-            const T* src = reinterpret_cast<const T*>(g.in[i].data) + w.b * g.in[i].sb + w.t * g.in[i].st;
-            const T* grad = reinterpret_cast<const T*>(g.grad[i].data) + w.b * g.grad[i].sb + w.t * g.grad[i].st;
-            T* dst = reinterpret_cast<T*>(g.out[i].data) + w.b * g.out[i].sb + w.t * g.out[i].st;
-            for (int h = h0; h < h1; h += kRows) {
-                float a[kRows][4], b[kRows][4], x[kRows][4], y[kRows][4];
+            if (g.heads[i] == 0) continue;
+            const int rows = tile_rows(g, w, i);
+            for (int r = slot; r < rows; r += kSlots * kRows) {
+                float a[kRows][4], b[kRows][4], y[kRows][4], z[kRows][4];
+                Row x[kRows];
 #pragma unroll
                 for (int u = 0; u < kRows; ++u) {
-                    const int hu = min(h + u, h1 - 1);
-                    load_row<T, IL>(src + hu * g.in[i].sh, d, a[u], b[u]);
-                    load_row<T, IL>(grad + hu * g.grad[i].sh, d, x[u], y[u]);
+                    x[u] = row_of(g, i, min(r + u * kSlots, rows - 1));
+                    const Row there{min(x[u].j, w.tokens - 1), x[u].h};
+                    load_row<T, IL>(row_at<T>(g.in[i], w, there), d, a[u], b[u]);
+                    load_row<T, IL>(row_at<T>(g.grad[i], w, there), d, y[u], z[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < kRows; ++u) {
-                    float sq = 0.0f, ax = 0.0f, pa[4], pb[4];
+                    float c[4], s[4], sq = 0.0f, ax = 0.0f, pa[4], pb[4];
+                    lane_angles(angles, min(x[u].j, w.tokens - 1), lane, turned, c, s);  // s is the inverse rotation's
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        pa[e] = x[u][e] * c[e] - y[u][e] * s[e];  // s is the inverse rotation's
-                        pb[e] = x[u][e] * s[e] + y[u][e] * c[e];
+                        pa[e] = y[u][e] * c[e] - z[u][e] * s[e];
+                        pb[e] = y[u][e] * s[e] + z[u][e] * c[e];
                         sq = fmaf(a[u][e], a[u][e], fmaf(b[u][e], b[u][e], sq));
-                        ax = fmaf(pa[e] * wa[e], a[u][e], fmaf(pb[e] * wb[e], b[u][e], ax));
+                        ax = fmaf(pa[e] * wa[i][e], a[u][e], fmaf(pb[e] * wb[i][e], b[u][e], ax));
                     }
                     sq = group_sum<LP>(live ? sq : 0.0f);
                     ax = group_sum<LP>(live ? ax : 0.0f);
-                    if (!live || h + u >= h1) continue;
-                    const float r = 1.0f / sqrtf(fmaf(sq, inv_d, g.eps));
-                    const float m = ax * r * inv_d;  // mean(a n)
+                    if (!live || r + u * kSlots >= rows || x[u].j >= w.tokens) continue;
+                    const float n = rsqrtf(fmaf(sq, inv_d, g.eps));
+                    const float m = ax * n * inv_d;  // mean(a n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float na = a[u][e] * r, nb = b[u][e] * r;
+                        const float na = a[u][e] * n, nb = b[u][e] * n;
                         da[i][e] = fmaf(pa[e], na, da[i][e]);
                         db[i][e] = fmaf(pb[e], nb, db[i][e]);
-                        x[u][e] = r * (pa[e] * wa[e] - na * m);
-                        y[u][e] = r * (pb[e] * wb[e] - nb * m);
+                        y[u][e] = n * (pa[e] * wa[i][e] - na * m);
+                        z[u][e] = n * (pb[e] * wb[i][e] - nb * m);
                     }
-                    store_row<T, IL>(dst + (h + u) * g.out[i].sh, d, x[u], y[u]);
+                    store_row<T, IL>(row_at<T>(g.out[i], w, x[u]), d, y[u], z[u]);
                 }
             }
         }
@@ -297,8 +348,13 @@ __global__ __launch_bounds__(64) void norm_rope_weights_kernel(const float* part
     const int dim = blockIdx.x - i * head_dim;
     void* dst = i == 0 ? dq : dk;
     if (!dst) return;
+    const float* src = partial + ((int64_t)i * head_dim + dim) * parts;
+    float x[kNormRopeParts / 64];  // all loads at once
+#pragma unroll
+    for (int j = 0; j < kNormRopeParts / 64; ++j) x[j] = (int)threadIdx.x + 64 * j < parts ? src[threadIdx.x + 64 * j] : 0.0f;
     double sum = 0.0;
-    for (int j = threadIdx.x; j < parts; j += 64) sum += partial[((int64_t)i * head_dim + dim) * parts + j];
+#pragma unroll
+    for (int j = 0; j < kNormRopeParts / 64; ++j) sum += x[j];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (threadIdx.x != 0) return;
@@ -310,9 +366,7 @@ __global__ __launch_bounds__(64) void norm_rope_weights_kernel(const float* part
 
 template <typename T, int LP>
 int launch_lp(const NormRopeArgs& g, bool backward, hipStream_t stream) {
-    constexpr int64_t kMostBlocks = int64_t(1) << 20;  // more groups are walked with the grid's stride
-    const int64_t need = (g.groups + kThreads / LP - 1) / (kThreads / LP);
-    const int blocks = backward ? norm_rope_parts(g) : static_cast<int>(need < kMostBlocks ? need : kMostBlocks);
+    const int blocks = backward ? norm_rope_parts(g) : static_cast<int>(g.tiles);
     if (backward) {
         if (g.rope.interleaved)
             hipLaunchKernelGGL((norm_rope_backward_kernel<T, LP, true>), dim3(blocks), dim3(kThreads), 0, stream, g);
@@ -345,27 +399,28 @@ int launch_t(const NormRopeArgs& g, bool backward, hipStream_t stream) {
 // Lanes that hold a row.
 int norm_rope_lanes(int head_dim) { return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32; }
 
-// A group takes as many of a token's rows as leave about eight waves per SIMD:
-// the angles of a token cost about as much as two of its rows.
+// Tiles of up to 16 tokens (a power of two), as large as leaves 4096 workgroups.
 void norm_rope_split(NormRopeArgs& g) {
-    constexpr int64_t kWaves = 8 * 1024;
-    const int rows = g.heads[0] + g.heads[1];
+    constexpr int64_t kWorkgroups = 4096;
     const int64_t tokens = (int64_t)g.batch * g.tokens;
-    const int64_t want = kWaves * (64 / norm_rope_lanes(g.head_dim));
-    int64_t per_token = (want + tokens - 1) / tokens;
-    if (per_token > rows) per_token = rows;
-    g.rows_per_group = static_cast<int>((rows + per_token - 1) / per_token);
-    g.groups_per_token = (rows + g.rows_per_group - 1) / g.rows_per_group;
-    g.groups = tokens * g.groups_per_token;
+    g.tile_tokens = 1;
+    g.tile_shift = 0;
+    while (g.tile_tokens < kTileTokens && tokens >= 2 * g.tile_tokens * kWorkgroups && g.heads[0] + g.heads[1] <= 4096) {
+        g.tile_tokens *= 2;
+        ++g.tile_shift;
+    }
+    g.tiles_per_batch = (g.tokens + g.tile_tokens - 1) / g.tile_tokens;
+    g.tiles = (int64_t)g.batch * g.tiles_per_batch;
+    for (int i = 0; i < 2; ++i) {
+        // the smaller step in memory first
+        g.heads_first[i] = g.heads[i] > 1 && llabs(g.in[i].sh) <= llabs(g.in[i].st);
+        g.inv_heads[i] = g.heads[i] > 1 ? static_cast<uint32_t>(((int64_t(1) << 32) + g.heads[i] - 1) / g.heads[i]) : 0;
+    }
 }
 
 // Workgroups of the backward pass: at most four per CU, which leaves one
 // partial weight gradient each.
-int norm_rope_parts(const NormRopeArgs& g) {
-    const int64_t slots = kThreads / norm_rope_lanes(g.head_dim);
-    const int64_t blocks = (g.groups + slots - 1) / slots;
-    return static_cast<int>(blocks < kNormRopeParts ? blocks : kNormRopeParts);
-}
+int norm_rope_parts(const NormRopeArgs& g) { return static_cast<int>(g.tiles < kNormRopeParts ? g.tiles : kNormRopeParts); }
 
 int launch_norm_rope(int dtype, const NormRopeArgs& g, bool backward, hipStream_t stream) {
     if (dtype == PISA_DTYPE_BF16) return launch_t<bf16_t>(g, backward, stream);
