@@ -1241,11 +1241,11 @@ int attn_hip_dense_backward(int32_t dtype, int32_t batch, int32_t heads, int32_t
         return rc;
     if (!lse || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(grad_lse) & 3))
         return fail(PISA_ERR_INVALID_ARGUMENT, "lse must be non-null, lse and grad_lse aligned to 4 bytes");
-    // the packing launch has a workgroup for every 64-row block of both sides
-    const int64_t blocks = (int64_t)batch * heads * (((int64_t)q_tokens + 63) / 64) +
-                           (int64_t)batch * kv_heads * (((int64_t)kv_tokens + 63) / 64);
+    // the packing launch has a workgroup for every 64-row block of q, grad_out, k and v
+    const int64_t blocks = 2 * ((int64_t)batch * heads * (((int64_t)q_tokens + 63) / 64) +
+                                (int64_t)batch * kv_heads * (((int64_t)kv_tokens + 63) / 64));
     if (blocks > kMaxGridBlocks)
-        return fail(PISA_ERR_UNSUPPORTED, "dense_backward supports %lld 64-row blocks of queries and keys over all heads, got %lld",
+        return fail(PISA_ERR_UNSUPPORTED, "dense_backward supports %lld 64-row blocks of q, grad_out, k and v over all heads, got %lld",
                     (long long)kMaxGridBlocks, (long long)blocks);
     pisa::BackwardArgs a;
     memset(&a, 0, sizeof(a));

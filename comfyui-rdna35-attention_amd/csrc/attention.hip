@@ -66,19 +66,23 @@ template <bool TRAIN> using ArgsFor = std::conditional_t<TRAIN, AttnTrainArgs, A
 // second product: the backward pass forms them again from it, and a sum of
 // rounded values would be off by half a step of T where one key holds the row.
 // A batch entry with no key at all gives zero rows and minus infinity.
-template <typename T, int D, int NT, bool SPARSE, bool TAIL, bool PERSIST = false, bool TRAIN = false>
+// W > 1 (TRAIN): the W waves of a workgroup share one query block, each walking a
+// contiguous part (`wave`) of its chunks, possibly an empty one, and merge
+// through `merge` (W (MD NT 1024 + 64 NT) floats) in a fixed order.
+template <typename T, int D, int NT, bool SPARSE, bool TAIL, bool PERSIST = false, bool TRAIN = false, int W = 1>
 __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh, int qb, int sub,
                                                 const int32_t* __restrict__ sel,
                                                 const uint32_t* __restrict__ selmask,
                                                 lds_char* lds = nullptr, bool from_lds = false,
-                                                NextBlock next = NextBlock{0, 0, 0, 0}) {
+                                                NextBlock next = NextBlock{0, 0, 0, 0}, int wave = 0,
+                                                float* merge = nullptr) {
     static_assert(D % 32 == 0 && D <= 256, "padded head dim");
     static_assert(NT == 1 || (NT == 2 && D <= 128), "query tiles per wave");
     typedef typename Elem<T>::vec8 vec8;
     constexpr int KT = D / 16;
     constexpr int MD = D / 32;
     constexpr int64_t kBlockBytes = (int64_t)D * kBlock * sizeof(T);
-    int lane_id = threadIdx.x;
+    int lane_id = W > 1 ? threadIdx.x & 63 : threadIdx.x;
     // a persistent wave re-derives its lane terms per block rather than holding
     // every lane-dependent offset in registers across blocks
     if constexpr (PERSIST) asm volatile("" : "+v"(lane_id));
@@ -88,6 +92,7 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
     const float c = a.scale_log2;
     const bool all_dims = a.head_dim >= D;  // else dims past the real head dim read as zero
     static_assert(!TRAIN || (!SPARSE && !TAIL && !PERSIST), "the training forward is dense");
+    static_assert(W == 1 || TRAIN, "waves share a query block in the training forward only");
     int kv_tokens = a.kv_tokens, kv_bh = bh;
     if constexpr (TRAIN) {
         kv_bh = bh / a.kv_group;
@@ -183,7 +188,9 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
     }
 
     // ---- chunk list: [0, n_exact) exact blocks, [n_exact, n_chunks) centroid chunks
-    const int n_exact = SPARSE ? a.exact : TRAIN ? (kv_tokens + kBlock - 1) / kBlock : a.kv_blocks;
+    const int all_chunks = TRAIN ? (kv_tokens + kBlock - 1) / kBlock : 0;
+    const int first = W > 1 ? wave * all_chunks / W : 0;  // this wave's first chunk
+    const int n_exact = SPARSE ? a.exact : TRAIN ? (W > 1 ? (wave + 1) * all_chunks / W - first : all_chunks) : a.kv_blocks;
     const int n_chunks = n_exact + (TAIL ? a.npad / kBlock : 0);
     const int32_t* my_idx = SPARSE ? sel + ((int64_t)bh * a.q_blocks + qb) * a.exact : nullptr;
     const uint32_t* my_mask = TAIL ? selmask + ((int64_t)bh * a.q_blocks + qb) * a.mask_words : nullptr;
@@ -254,7 +261,7 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
     auto table_row = [&](int x) -> int {  // block id, or centroid chunk id for tail chunks
         x = min(x, n_chunks - 1);
         if (TAIL && x >= n_exact) return x - n_exact;
-        return SPARSE ? my_idx[x] : x;
+        return SPARSE ? my_idx[x] : first + x;
     };
     struct Src {
         __amdgpu_buffer_rsrc_t rs;
@@ -474,7 +481,7 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
         // cc + 2, or the last one re-read).
         auto chunk_step = [&](int cc, bool last, bool half0_only, int kind) __attribute__((always_inline)) {
             const bool exact_k = kind == kStepExact, tail_k = kind == kStepTail;
-            const int row2 = exact_k ? (SPARSE ? my_idx[cc + 2] : cc + 2) : table_row(cc + 2);
+            const int row2 = exact_k ? (SPARSE ? my_idx[cc + 2] : first + cc + 2) : table_row(cc + 2);
             const bool tail = tail_k || (!exact_k && is_tail(cc));
             const Src kn = (first_order && last) ? Src{ht_rs, 0}
                            : exact_k ? Src{kp_rs, row1 * (int)kBlockBytes}
@@ -546,6 +553,46 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
     // tile at a time (keeps only 32 extra accumulators live), store the real
     // head dims
     float inv[NT], wa[NT];
+    if constexpr (W > 1) {
+        // per column the parts' running maxima and sums, then O: each part scaled to
+        // the common maximum, summed in order by every wave
+        float* const stat = merge + W * MD * NT * 1024;
+        float top[NT], sum[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float lw = add_xor32(l[nt]);
+            if (half == 0) {
+                stat[((wave * NT + nt) * 2) * 32 + col] = lw > 0.0f || lw != lw ? -nm[nt] : -__builtin_inff();
+                stat[((wave * NT + nt) * 2 + 1) * 32 + col] = lw;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            top[nt] = -__builtin_inff();
+            sum[nt] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) top[nt] = __builtin_elementwise_maximum(top[nt], stat[((w * NT + nt) * 2) * 32 + col]);
+            const float base = top[nt] == -__builtin_inff() ? 0.0f : top[nt];
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                sum[nt] += stat[((w * NT + nt) * 2 + 1) * 32 + col] *
+                           __builtin_amdgcn_exp2f(stat[((w * NT + nt) * 2) * 32 + col] - base);
+            const float f = __builtin_amdgcn_exp2f(stat[((wave * NT + nt) * 2) * 32 + col] - base);
+#pragma unroll
+            for (int md = 0; md < MD; ++md)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = o[md][nt][4 * g + e] * f;
+                    *reinterpret_cast<f32x4*>(&merge[((((wave * MD + md) * NT + nt) * 4 + g) * 64 + lane) * 4]) = x;
+                }
+            nm[nt] = -base;
+            l[nt] = half == 0 ? sum[nt] : 0.0f;
+        }
+        __syncthreads();
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const float lf = add_xor32(l[nt]);
@@ -553,10 +600,10 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
         inv[nt] = 1.0f / lf;
         wa[nt] = ltf * inv[nt] * a.corr_scale;
         if constexpr (TRAIN) {
-            if (n_chunks == 0) inv[nt] = 0.0f;
+            if (all_chunks == 0) inv[nt] = 0.0f;
             const int row = qb * kBlock + 32 * (sub + nt) + col;
-            if (half == 0 && row < a.q_tokens)
-                a.lse[(int64_t)bh * a.q_tokens + row] = n_chunks == 0 ? -__builtin_inff() : (__builtin_log2f(lf) - nm[nt]) * kLn2;
+            if (half == 0 && row < a.q_tokens && wave == 0)
+                a.lse[(int64_t)bh * a.q_tokens + row] = all_chunks == 0 ? -__builtin_inff() : (__builtin_log2f(lf) - nm[nt]) * kLn2;
         }
     }
     char* obase[NT];
@@ -578,6 +625,20 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
                       ((a.o.sb | a.o.sh | a.o.st) * (int64_t)sizeof(T)) % 16 == 0;
 #pragma unroll
     for (int md = 0; md < MD; ++md) {
+        if constexpr (W > 1) {
+            if (md % W != wave) continue;  // a tile of 32 dims is stored by one wave
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int w = 0; w < W; ++w)
+                        x += *reinterpret_cast<const f32x4*>(&merge[((((w * MD + md) * NT + nt) * 4 + g) * 64 + lane) * 4]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[md][nt][4 * g + e] = x[e];
+                }
+        }
         f32x16 corr[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -695,6 +756,24 @@ void attention_kernel(ArgsFor<TRAIN> a, const int32_t* __restrict__ sel, const u
     }
     attention_block<T, D, NT, SPARSE, TAIL, false, TRAIN>(a, bh, block_work - bh * a.q_blocks,
                                                           work - block_work * SUBS, sel, selmask, qbuf);
+}
+
+// Small training forwards: W waves to a work item of attention_kernel.
+template <typename T, int D, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void attention_shared_kernel(AttnTrainArgs a) {
+    constexpr int NT = D <= 128 ? 2 : 1, SUBS = 2 / NT;
+    constexpr int kMerge = W * (D / 32 * NT * 1024 + 64 * NT) * 4, kQuery = D > 192 ? W * (D / 16) * 1024 : 0;
+    // the query fragments of D = 256 (QLDS) are read for the last time before the merge
+    __shared__ __attribute__((aligned(1024))) char buf[kMerge > kQuery ? kMerge : kQuery];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int work = xcd_remap(blockIdx.x, gridDim.x);
+    const int block_work = work / SUBS;
+    const int bh = block_work / a.q_blocks;
+    attention_block<T, D, NT, false, false, false, true, W>(
+        a, bh, block_work - bh * a.q_blocks, work - block_work * SUBS, nullptr, nullptr,
+        kQuery ? (lds_char*)buf + wave * (D / 16) * 1024 : nullptr, false, NextBlock{0, 0, 0, 0}, wave,
+        reinterpret_cast<float*>(buf));
 }
 
 // Persistent variant (D = 128, head dim 128, a grid that splits evenly into the
@@ -926,16 +1005,37 @@ int launch_attention_t(const ArgsFor<TRAIN>& a_in, int bh_count, hipStream_t str
     X(bf16_t, 64) X(bf16_t, 96) X(bf16_t, 128) X(bf16_t, 160) X(bf16_t, 192) X(bf16_t, 256) \
     X(f16_t, 64) X(f16_t, 96) X(f16_t, 128) X(f16_t, 160) X(f16_t, 192) X(f16_t, 256)
 #if defined(PISA_ATTENTION_TRAIN)
-// attention_train.hip: the dense kernels' training variant, under the same scheduler
+// attention_train.hip: the dense kernels' training variant, under the same scheduler.
+// Work items that leave SIMDs idle are shared by two or four waves each, where the
+// rounds of the SIMDs times a wave's chunks (and about four chunks' time for a
+// merge) come out smaller: [1,8,1000,64] 19.2 -> 10.5 us with four.
+template <typename T, int D>
+static int launch_train_d(const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
+    constexpr int kSubs = D <= 128 ? 1 : 2;
+    const int items = bh_count * a.q_blocks * kSubs;
+    const int simds = 8 * xcd_slots();
+    auto cost = [&](int w) {
+        return ((int64_t)items * w + simds - 1) / simds * ((a.kv_blocks + w - 1) / w + (w > 1 ? 4 : 0));
+    };
+    if (simds > 0 && cost(4) < cost(1) && cost(4) <= cost(2)) {
+        hipLaunchKernelGGL((attention_shared_kernel<T, D, 4>), dim3(items), dim3(256), 0, stream, a);
+        return pisa_host::check_launch("attention_shared_kernel");
+    }
+    if (simds > 0 && cost(2) < cost(1)) {
+        hipLaunchKernelGGL((attention_shared_kernel<T, D, 2>), dim3(items), dim3(128), 0, stream, a);
+        return pisa_host::check_launch("attention_shared_kernel");
+    }
+    return launch_attention_t<T, D, false, false, true>(a, bh_count, stream);
+}
 template <typename T>
 static int launch_train_t(int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
     switch (padded) {
-        case 64: return launch_attention_t<T, 64, false, false, true>(a, bh_count, stream);
-        case 96: return launch_attention_t<T, 96, false, false, true>(a, bh_count, stream);
-        case 128: return launch_attention_t<T, 128, false, false, true>(a, bh_count, stream);
-        case 160: return launch_attention_t<T, 160, false, false, true>(a, bh_count, stream);
-        case 192: return launch_attention_t<T, 192, false, false, true>(a, bh_count, stream);
-        case 256: return launch_attention_t<T, 256, false, false, true>(a, bh_count, stream);
+        case 64: return launch_train_d<T, 64>(a, bh_count, stream);
+        case 96: return launch_train_d<T, 96>(a, bh_count, stream);
+        case 128: return launch_train_d<T, 128>(a, bh_count, stream);
+        case 160: return launch_train_d<T, 160>(a, bh_count, stream);
+        case 192: return launch_train_d<T, 192>(a, bh_count, stream);
+        case 256: return launch_train_d<T, 256>(a, bh_count, stream);
         default: return pisa_host::fail(PISA_ERR_UNSUPPORTED, "training attention: padded head dim %d", padded);
     }
 }

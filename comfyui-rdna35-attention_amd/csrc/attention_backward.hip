@@ -151,22 +151,30 @@ template <typename T, int D> __device__ __forceinline__ float largest_row(const 
     return s;
 }
 
-// Workgroups [0, q_work): query blocks (Q, dO, O); the rest: key blocks (K, V).
+// One workgroup per 64-row block of one tensor: dO (with O), Q, K, V.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardArgs a) {
     constexpr int KT = D / 16;
+    constexpr int64_t kQBytes = q_unit_frags<D>() * 1024, kKvBytes = kv_unit_frags<D>() * 1024;
     __shared__ __attribute__((aligned(16))) PackLds<T, D> lds;
     const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
-    const int q_work = a.batch * a.heads * q_blocks;
+    const int q_work = a.batch * a.heads * q_blocks, kv_work = a.batch * a.k.heads * kv_blocks;
     const int t = threadIdx.x;
-    if ((int)blockIdx.x < q_work) {
-        constexpr int64_t kBytes = q_unit_frags<D>() * 1024;
-        const int bh = blockIdx.x / q_blocks;
-        const int j = blockIdx.x - bh * q_blocks;
+    const bool q_side = (int)blockIdx.x < 2 * q_work;
+    const int item = q_side ? blockIdx.x : blockIdx.x - 2 * q_work;
+    const bool second = item >= (q_side ? q_work : kv_work);
+    const int block = second ? item - (q_side ? q_work : kv_work) : item;
+    const int bh = block / (q_side ? q_blocks : kv_blocks);
+    const int j = block - bh * (q_side ? q_blocks : kv_blocks);
+    auto rows = [&](const View& v) { return v.data + v.row(bh, (int64_t)j * kBlock) * (int64_t)sizeof(T); };
+    if (q_side) {
         const int live = a.q_tokens - j * kBlock, last = live - 1;
-        char* units = a.qx + ((int64_t)bh * a.q_units + 2 * j) * kBytes;
-        auto rows = [&](const View& v) { return v.data + v.row(bh, (int64_t)j * kBlock) * (int64_t)sizeof(T); };
-        pack_block<T, D>(lds, rows(a.dout), a.dout.st, rows(a.o), a.o.st, live, last, a.head_dim, units, kBytes, KT, 2 * KT,
+        char* units = a.qx + ((int64_t)bh * a.q_units + 2 * j) * kQBytes;
+        if (second) {
+            pack_block<T, D>(lds, rows(a.q), a.q.st, nullptr, 0, live, last, a.head_dim, units, kQBytes, 0, 3 * KT, false);
+            return;
+        }
+        pack_block<T, D>(lds, rows(a.dout), a.dout.st, rows(a.o), a.o.st, live, last, a.head_dim, units, kQBytes, KT, 2 * KT,
                          kScaled<T>);
         if (t < kBlock) {
             float delta = 0.0f;
@@ -175,7 +183,7 @@ __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardAr
             const int64_t at = (int64_t)bh * a.q_tokens + (int64_t)j * kBlock + t;
             const float dlse = valid && a.dlse ? a.dlse[at] : 0.0f;
             const float nl = valid ? (kScaled<T> ? kShift16 : 0.0f) - a.lse[at] * kLog2e : -__builtin_inff();
-            float* stat = reinterpret_cast<float*>(units + (t >> 5) * kBytes + 4 * KT * 1024);
+            float* stat = reinterpret_cast<float*>(units + (t >> 5) * kQBytes + 4 * KT * 1024);
             stat[t & 31] = nl;
             stat[32 + (t & 31)] = dlse - delta;
             if constexpr (kScaled<T>) {
@@ -189,19 +197,15 @@ __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardAr
                 }
             }
         }
-        __syncthreads();
-        pack_block<T, D>(lds, rows(a.q), a.q.st, nullptr, 0, live, last, a.head_dim, units, kBytes, 0, 3 * KT, false);
     } else {
-        constexpr int64_t kBytes = kv_unit_frags<D>() * 1024;
-        const int work = blockIdx.x - q_work;
-        const int bh = work / kv_blocks;
-        const int j = work - bh * kv_blocks;
         const int last = a.kv_tokens - j * kBlock - 1;
         const int live = a.length(bh / a.k.heads) - j * kBlock;
-        char* units = a.kx + ((int64_t)bh * a.kv_units + 2 * j) * kBytes;
-        auto rows = [&](const View& v) { return v.data + v.row(bh, (int64_t)j * kBlock) * (int64_t)sizeof(T); };
-        pack_block<T, D>(lds, rows(a.k), a.k.st, nullptr, 0, live, last, a.head_dim, units, kBytes, 0, 2 * KT, false);
-        pack_block<T, D>(lds, rows(a.v), a.v.st, nullptr, 0, live, last, a.head_dim, units, kBytes, KT, -1, kScaled<T>);
+        char* units = a.kx + ((int64_t)bh * a.kv_units + 2 * j) * kKvBytes;
+        if (!second) {
+            pack_block<T, D>(lds, rows(a.k), a.k.st, nullptr, 0, live, last, a.head_dim, units, kKvBytes, 0, 2 * KT, false);
+            return;
+        }
+        pack_block<T, D>(lds, rows(a.v), a.v.st, nullptr, 0, live, last, a.head_dim, units, kKvBytes, KT, -1, kScaled<T>);
         if constexpr (kScaled<T>) {
             if (t < kBlock) {
                 const float most = largest_row<T, D>(lds);
@@ -280,17 +284,27 @@ __device__ __forceinline__ float shift_of(float bound) {
     return static_cast<float>(__builtin_amdgcn_readfirstlane(exponent));
 }
 
-// Largest of n values by the whole workgroup, the same in every thread.
-__device__ __forceinline__ float largest(const float* x, int n, float* scratch) {
-    float m = 0.0f;
-    for (int i = threadIdx.x; i < n; i += 64 * kWaves) m = fmaxf(m, x[i]);
+// The largest of each of three arrays by the whole workgroup, combined into
+// dS's bound, the same in every thread.
+__device__ __forceinline__ float bound_of(const float* most_o, int n_o, const float* most_v, int n_v, const float* most_l) {
+    __shared__ float scratch[3][kWaves];
+    float m[3] = {0.0f, 0.0f, 0.0f};
+    for (int i = threadIdx.x; i < n_o; i += 64 * kWaves) {
+        m[0] = fmaxf(m[0], most_o[i]);
+        m[2] = fmaxf(m[2], most_l[i]);
+    }
+    for (int i = threadIdx.x; i < n_v; i += 64 * kWaves) m[1] = fmaxf(m[1], most_v[i]);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) m[j] = fmaxf(m[j], __shfl_xor(m[j], o));
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) scratch[j][threadIdx.x >> 6] = m[j];
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = m;
-    __syncthreads();
-    const float all = fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3]));
-    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(all)));  // a scalar register
+#pragma unroll
+    for (int j = 0; j < 3; ++j) m[j] = fmaxf(fmaxf(scratch[j][0], scratch[j][1]), fmaxf(scratch[j][2], scratch[j][3]));
+    return fmaf(2.0f * m[0], m[1], m[2]);
 }
 
 // Stores 32 dims of one row per lane pair: x[v] is dim 8(v/4) + 4half + v%4 of
@@ -374,13 +388,20 @@ __global__ __launch_bounds__(64) void attention_backward_join_kernel(const float
     f32x16 x;
 #pragma unroll
     for (int v = 0; v < 16; ++v) x[v] = 0.0f;
-    for (int i = 0; i < p.parts; ++i)
+    constexpr int kBatch = 4;  // parts whose loads go out together
+    for (int i0 = 0; i0 < p.parts; i0 += kBatch) {
+        f32x4 y[kBatch][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 y = *reinterpret_cast<const f32x4*>(src + i * slots + q * 256);
+        for (int i = 0; i < kBatch; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * q + e] += y[e];
-        }
+            for (int q = 0; q < 4; ++q)
+                y[i][q] = *reinterpret_cast<const f32x4*>(src + min(i0 + i, p.parts - 1) * slots + q * 256);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (i0 + i < p.parts)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[v] += y[i][v / 4][v % 4];
+    }
     const OutView& out = tensor == 0 ? out0 : out1;
     const int token = unit * kUnit + (lane & 31);
     if (token < tokens)
@@ -392,7 +413,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void attention_backward_kv_kernel(BackwardArgs a) {
     typedef typename Elem<T>::vec8 vec8;
-    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = q_unit_frags<D>(), S = stages<D>(), R = 4;
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = q_unit_frags<D>(), S = stages<D>(), R = D > 128 && D < 256 ? 8 : 4;
     constexpr int kBytes = FRAGS * 1024;
     __shared__ __attribute__((aligned(1024))) char lds_buf[S * kBytes];
     lds_char* const lds = (lds_char*)lds_buf;
@@ -417,18 +438,12 @@ void attention_backward_kv_kernel(BackwardArgs a) {
         return table + ((int64_t)h * a.q_units + (i - h * q_live)) * kBytes;
     };
 
-    float e = 0.0f;  // log2 of dS's factor
-    if constexpr (kScaled<T>) {
-        float* scratch = reinterpret_cast<float*>(lds_buf);
-        const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
-        const float mo = largest(a.q_most + (int64_t)bh * a.kv_group * q_blocks, a.kv_group * q_blocks, scratch);
-        const float ml = largest(a.l_most + (int64_t)bh * a.kv_group * q_blocks, a.kv_group * q_blocks, scratch);
-        const float mv = largest(a.v_most + (int64_t)bh * kv_blocks, kv_blocks, scratch);
-        e = shift_of(fmaf(2.0f * mo, mv, ml));
-        __syncthreads();
+    // the first units are on their way to LDS while the own operands are read
+    const uint32_t base = (uint32_t)(uintptr_t)lds;
+    if (i0 < i1) {
+        copy_unit<FRAGS>(unit_of(i0), base, wave, lane * 16);
+        if constexpr (S == 3) copy_unit<FRAGS>(unit_of(i0 + 1), base + kBytes, wave, lane * 16);
     }
-    const float f = __builtin_amdgcn_exp2f(e - kShift16);
-
     constexpr int NV = kValuesInLds<D> ? N - 1 : N;
     __shared__ __attribute__((aligned(1024))) char own_buf[kValuesInLds<D> ? kWaves * KT * 1024 : 16];
     lds_char* const own_v = (lds_char*)own_buf + (kValuesInLds<D> ? wave * KT * 1024 + lane * 16 : 0);
@@ -447,6 +462,13 @@ void attention_backward_kv_kernel(BackwardArgs a) {
                 *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(own_v + t * 1024) = __builtin_bit_cast(u32x4, x);
         }
     }
+    float e = 0.0f;  // log2 of dS's factor
+    if constexpr (kScaled<T>) {
+        const int q_blocks = a.kv_group * (a.q_units / 2), kv_blocks = a.kv_units / 2;
+        e = shift_of(bound_of(a.q_most + (int64_t)bh * q_blocks, q_blocks, a.v_most + (int64_t)bh * kv_blocks, kv_blocks,
+                              a.l_most + (int64_t)bh * q_blocks));
+    }
+    const float f = __builtin_amdgcn_exp2f(e - kShift16);
     f32x16 dk[N][MD], dv[N][MD];
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -456,10 +478,7 @@ void attention_backward_kv_kernel(BackwardArgs a) {
             for (int v = 0; v < 16; ++v) dk[n][md][v] = dv[n][md][v] = 0.0f;
 
     if (i0 < i1) {
-        const uint32_t base = (uint32_t)(uintptr_t)lds;
-        __builtin_amdgcn_s_waitcnt(kWaitVm0);  // the own operands: only copies are in flight from here on
-        copy_unit<FRAGS>(unit_of(i0), base, wave, lane * 16);
-        if constexpr (S == 3) copy_unit<FRAGS>(unit_of(i0 + 1), base + kBytes, wave, lane * 16);
+        __builtin_amdgcn_s_waitcnt(kWaitVm0);  // the own operands have landed too: only copies are in flight from here on
         wait_copies();
         vec8 ring[R];  // the next fragments, read R steps ahead
 #pragma unroll
@@ -564,7 +583,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void attention_backward_q_kernel(BackwardArgs a) {
     typedef typename Elem<T>::vec8 vec8;
-    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kv_unit_frags<D>(), S = 3, R = 6;
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kv_unit_frags<D>(), S = 3, R = D <= 128 ? 6 : D == 160 ? 10 : 12;
     constexpr int kBytes = FRAGS * 1024;
     __shared__ __attribute__((aligned(1024))) char lds_buf[S * kBytes];
     lds_char* const lds = (lds_char*)lds_buf;
@@ -584,30 +603,35 @@ void attention_backward_q_kernel(BackwardArgs a) {
     // fragment of the buffer used j-th: K rows, K^T, V rows
     auto order = [](int j) { return j < KT ? j : j < 2 * KT ? j + KT : j - KT; };
 
-    float e = 0.0f;
-    if constexpr (kScaled<T>) {
-        float* scratch = reinterpret_cast<float*>(lds_buf);
-        const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
-        const float mo = largest(a.q_most + (int64_t)bh * q_blocks, q_blocks, scratch);
-        const float ml = largest(a.l_most + (int64_t)bh * q_blocks, q_blocks, scratch);
-        const float mv = largest(a.v_most + (int64_t)kv_bh * kv_blocks, kv_blocks, scratch);
-        e = shift_of(fmaf(2.0f * mo, mv, ml));
-        __syncthreads();
+    const uint32_t base = (uint32_t)(uintptr_t)lds;
+    auto copy_step = [&](int i, int b) {
+        copy_unit<FRAGS, 2 * KT>(unit_of(i), unit_of(max(i - 1, i0)), base + b * kBytes, wave, lane * 16);
+    };
+    if (i0 < i1) {
+        copy_step(i0, 0);
+        copy_step(i0 + 1, 1);
     }
-
     vec8 qf[N][KT], of[N][KT];
     float nl[N], nd[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const char* own = a.qx + ((int64_t)bh * a.q_units + min(unit0 + n, a.q_units - 1)) * (q_unit_frags<D>() * 1024);
         const float* stat = reinterpret_cast<const float*>(own + 4 * KT * 1024);
-        nl[n] = stat[col] + (kScaled<T> ? e - kShift16 : 0.0f);
+        nl[n] = stat[col];
         nd[n] = stat[32 + col];
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             qf[n][t] = load8<vec8>(own + t * 1024 + lane * 16);
             of[n][t] = load8<vec8>(own + (KT + t) * 1024 + lane * 16);
         }
+    }
+    float e = 0.0f;  // log2 of dS's factor
+    if constexpr (kScaled<T>) {
+        const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
+        e = shift_of(bound_of(a.q_most + (int64_t)bh * q_blocks, q_blocks, a.v_most + (int64_t)kv_bh * kv_blocks, kv_blocks,
+                              a.l_most + (int64_t)bh * q_blocks));
+#pragma unroll
+        for (int n = 0; n < N; ++n) nl[n] += e - kShift16;
     }
     f32x16 dq[N][MD];
 #pragma unroll
@@ -618,16 +642,10 @@ void attention_backward_q_kernel(BackwardArgs a) {
             for (int v = 0; v < 16; ++v) dq[n][md][v] = 0.0f;
 
     // Step i forms S and dP of unit i and adds unit i - 1 to dQ: dS of i - 1 is formed
-    // beside the products of S, the probabilities of i beside those of dQ.  The
-    // buffer of step i therefore holds K and V rows of unit i and K^T of i - 1.
+    // beside the products of S, the probabilities of i beside those of dQ.  (The
+    // buffer of step i therefore holds K and V rows of unit i and K^T of i - 1.)
     if (i0 < i1) {
-        const uint32_t base = (uint32_t)(uintptr_t)lds;
-        auto copy_step = [&](int i, int b) {
-            copy_unit<FRAGS, 2 * KT>(unit_of(i), unit_of(max(i - 1, i0)), base + b * kBytes, wave, lane * 16);
-        };
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
-        copy_step(i0, 0);
-        copy_step(i0 + 1, 1);
         wait_copies();
         vec8 ring[R];
 #pragma unroll
@@ -722,7 +740,7 @@ int launch_t(const BackwardArgs& a, hipStream_t stream) {
     constexpr int MD = D / 32, kTile = kWaves * columns<D>();
     const int bh = a.batch * a.heads, kv_bh = a.batch * a.k.heads;
     int rc;
-    hipLaunchKernelGGL((attention_backward_pack_kernel<T, D>), dim3(bh * (a.q_units / 2) + kv_bh * (a.kv_units / 2)), dim3(256),
+    hipLaunchKernelGGL((attention_backward_pack_kernel<T, D>), dim3(bh * a.q_units + kv_bh * a.kv_units), dim3(256),
                        0, stream, a);
     if ((rc = pisa_host::check_launch("attention_backward_pack_kernel"))) return rc;
     auto workgroups = [](const BackwardTiles& p) { return dim3(p.whole + p.rest * p.parts); };

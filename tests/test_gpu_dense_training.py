@@ -75,6 +75,10 @@ CASES = [
     ((1, 4, 1, 40, 2500, 72), None),        # few queries: the keys are split
     ((4, 64, 64, 65, 65, 64), None),        # as many workgroups as CUs: no split
     ((1, 1, 1, 640, 640, 128), None),
+    ((2, 2, 2, 65, 900, 160), [70, 833]),   # waves that share a query block, some of them without a key
+    ((3, 1, 1, 40, 1000, 256), [0, 64, 1000]),
+    ((4, 2, 1, 100, 1100, 64), [1, 129, 0, 1024]),
+    ((2, 2, 1, 70, 1500, 96), [1500, 333]),
 ]
 
 
