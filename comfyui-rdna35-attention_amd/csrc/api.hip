@@ -1200,9 +1200,10 @@ int attn_hip_dense_forward_lse(int32_t dtype, int32_t batch, int32_t heads, int3
 }
 
 static int64_t carve_backward(int dtype, int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int head_dim,
-                              void* workspace, pisa::BackwardArgs& a) {
-    const pisa::BackwardPlan p = pisa::plan_backward(batch, heads, kv_heads, q_tokens, kv_tokens,
-                                                     pisa::padded_head_dim(head_dim), dtype == PISA_DTYPE_F16);
+                              bool with_q, bool with_kv, void* workspace, pisa::BackwardArgs& a) {
+    const pisa::BackwardPlan p =
+        pisa::plan_backward(batch, heads, kv_heads, q_tokens, kv_tokens, pisa::padded_head_dim(head_dim),
+                            dtype == PISA_DTYPE_F16, with_q, with_kv);
     a.q_units = p.q_units;
     a.kv_units = p.kv_units;
     a.q_tiles = p.q_tiles;
@@ -1213,16 +1214,23 @@ static int64_t carve_backward(int dtype, int batch, int heads, int kv_heads, int
     a.q_most = c.take<float>(p.q_most_bytes);
     a.v_most = c.take<float>(p.v_most_bytes);
     a.l_most = c.take<float>(p.l_most_bytes);
-    a.part = c.take<float>(p.part_bytes);
+    a.q_part = c.take<float>(p.q_part_bytes);
+    a.kv_part = c.take<float>(p.kv_part_bytes);
     return c.off;
 }
 
 int64_t attn_hip_dense_backward_workspace_bytes(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads,
                                                 int32_t q_tokens, int32_t kv_tokens, int32_t head_dim) {
     if (check_train("dense_backward", dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, 1.0f, nullptr)) return 0;
-    pisa::BackwardArgs a;
-    memset(&a, 0, sizeof(a));
-    return carve_backward(dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, nullptr, a);
+    // the largest of all gradients, dq alone, dk and dv alone, which split their work differently
+    int64_t most = 0;
+    for (int i = 1; i < 4; ++i) {
+        pisa::BackwardArgs a;
+        memset(&a, 0, sizeof(a));
+        most = std::max(most, carve_backward(dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, i & 1, i & 2,
+                                             nullptr, a));
+    }
+    return most;
 }
 
 int attn_hip_dense_backward(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens,
@@ -1249,7 +1257,8 @@ int attn_hip_dense_backward(int32_t dtype, int32_t batch, int32_t heads, int32_t
                     (long long)kMaxGridBlocks, (long long)blocks);
     pisa::BackwardArgs a;
     memset(&a, 0, sizeof(a));
-    const int64_t need = carve_backward(dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, workspace, a);
+    const int64_t need = carve_backward(dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, dq.data != nullptr,
+                                        dk.data != nullptr, workspace, a);
     if (!workspace_ok(workspace, workspace_bytes, need))
         return fail(PISA_ERR_WORKSPACE, "workspace of %lld bytes required, got %lld", (long long)need,
                     (long long)workspace_bytes);

@@ -1008,7 +1008,8 @@ int launch_attention_t(const ArgsFor<TRAIN>& a_in, int bh_count, hipStream_t str
 // attention_train.hip: the dense kernels' training variant, under the same scheduler.
 // Work items that leave SIMDs idle are shared by two or four waves each, where the
 // rounds of the SIMDs times a wave's chunks (and about four chunks' time for a
-// merge) come out smaller: [1,8,1000,64] 19.2 -> 10.5 us with four.
+// merge) come out smaller: [1,8,1000,64] 19.2 -> 10.5 us with four.  (Fuller grids
+// stay as they are: [2,16,9216,128] 1270-1300 us, 1304 with two.)
 template <typename T, int D>
 static int launch_train_d(const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
     constexpr int kSubs = D <= 128 ? 1 : 2;
@@ -1017,11 +1018,11 @@ static int launch_train_d(const AttnTrainArgs& a, int bh_count, hipStream_t stre
     auto cost = [&](int w) {
         return ((int64_t)items * w + simds - 1) / simds * ((a.kv_blocks + w - 1) / w + (w > 1 ? 4 : 0));
     };
-    if (simds > 0 && cost(4) < cost(1) && cost(4) <= cost(2)) {
+    if (items < simds && cost(4) < cost(1) && cost(4) <= cost(2)) {
         hipLaunchKernelGGL((attention_shared_kernel<T, D, 4>), dim3(items), dim3(256), 0, stream, a);
         return pisa_host::check_launch("attention_shared_kernel");
     }
-    if (simds > 0 && cost(2) < cost(1)) {
+    if (items < simds && cost(2) < cost(1)) {
         hipLaunchKernelGGL((attention_shared_kernel<T, D, 2>), dim3(items), dim3(128), 0, stream, a);
         return pisa_host::check_launch("attention_shared_kernel");
     }

@@ -286,8 +286,8 @@ __device__ __forceinline__ float shift_of(float bound) {
 
 // The largest of each of three arrays by the whole workgroup, combined into
 // dS's bound, the same in every thread.
-__device__ __forceinline__ float bound_of(const float* most_o, int n_o, const float* most_v, int n_v, const float* most_l) {
-    __shared__ float scratch[3][kWaves];
+__device__ __forceinline__ float bound_of(const float* most_o, int n_o, const float* most_v, int n_v, const float* most_l,
+                                          float (*scratch)[kWaves]) {
     float m[3] = {0.0f, 0.0f, 0.0f};
     for (int i = threadIdx.x; i < n_o; i += 64 * kWaves) {
         m[0] = fmaxf(m[0], most_o[i]);
@@ -338,9 +338,9 @@ template <typename T> __device__ __forceinline__ void store_tile(T* row, int d0,
 struct TileWork {
     int tile, part, parts, slot;  // slot: place among the fp32 parts (-1: whole)
 };
-__device__ __forceinline__ TileWork tile_work(const BackwardTiles& p) {
-    if ((int)blockIdx.x < p.whole) return TileWork{xcd_remap(blockIdx.x, p.whole), 0, 1, -1};
-    const int item = xcd_remap(blockIdx.x - p.whole, p.rest * p.parts);
+__device__ __forceinline__ TileWork tile_work(const BackwardTiles& p, int index) {
+    if (index < p.whole) return TileWork{xcd_remap(index, p.whole), 0, 1, -1};
+    const int item = xcd_remap(index - p.whole, p.rest * p.parts);
     const int part = item / p.rest, t = item - part * p.rest;
     return TileWork{p.whole + t, part, p.parts, p.parts > 1 ? item : -1};
 }
@@ -370,21 +370,25 @@ __device__ __forceinline__ void store_unit(const f32x16 (&g)[MD], float factor, 
 }
 
 // Sums the parts of the split tiles in order and stores their rows; one wave per
-// (tensor, tile, unit of the tile, 32 dims).
+// (tensor, tile, unit of the tile, 32 dims): dK, dV, then dQ.
 template <typename T, int MD, int UNITS>
-__global__ __launch_bounds__(64) void attention_backward_join_kernel(const float* part, BackwardTiles p, int units, int tokens,
-                                                                     int d_real, OutView out0, OutView out1) {
+__global__ __launch_bounds__(64) void attention_backward_join_kernel(BackwardArgs a) {
     const int lane = threadIdx.x;
     const int md = blockIdx.x % MD;
     int work = blockIdx.x / MD;
     const int u = work % UNITS;
     work /= UNITS;
+    const int kv_rest = a.kv_tiles.parts > 1 ? a.kv_tiles.rest : 0;
+    const bool q_side = work >= 2 * kv_rest;
+    const BackwardTiles& p = q_side ? a.q_tiles : a.kv_tiles;
+    work -= q_side ? 2 * kv_rest : 0;
     const int tensor = work / p.rest, t = work - tensor * p.rest;
     const int bh = (p.whole + t) / p.per_head;
     const int unit = ((p.whole + t) - bh * p.per_head) * UNITS + u;
-    if (unit >= units) return;
+    if (unit >= (q_side ? a.q_units : a.kv_units)) return;
     const int64_t slots = (int64_t)p.rest * UNITS * MD * 1024;  // floats of one part of one tensor
-    const float* src = part + tensor * p.parts * slots + (((int64_t)t * UNITS + u) * MD + md) * 1024 + lane * 4;
+    const float* src = (q_side ? a.q_part : a.kv_part) + tensor * p.parts * slots +
+                       (((int64_t)t * UNITS + u) * MD + md) * 1024 + lane * 4;
     f32x16 x;
 #pragma unroll
     for (int v = 0; v < 16; ++v) x[v] = 0.0f;
@@ -402,24 +406,29 @@ __global__ __launch_bounds__(64) void attention_backward_join_kernel(const float
 #pragma unroll
                 for (int v = 0; v < 16; ++v) x[v] += y[i][v / 4][v % 4];
     }
-    const OutView& out = tensor == 0 ? out0 : out1;
+    const OutView& out = q_side ? a.dq : tensor == 0 ? a.dk : a.dv;
     const int token = unit * kUnit + (lane & 31);
-    if (token < tokens)
-        store_tile<T>(reinterpret_cast<T*>(out.data) + out.row(bh, token), md * 32, d_real, x, lane >> 5);
+    if (token < (q_side ? a.q_tokens : a.kv_tokens))
+        store_tile<T>(reinterpret_cast<T*>(out.data) + out.row(bh, token), md * 32, a.head_dim, x, lane >> 5);
 }
+
+// LDS of a workgroup: the streamed units, at width 128 a part of the wave's own
+// values (kValuesInLds), and a few words to share.
+template <int D> constexpr int kv_lds_bytes() {
+    return stages<D>() * q_unit_frags<D>() * 1024 + (kValuesInLds<D> ? kWaves * (D / 16) * 1024 : 0);
+}
+constexpr int kQStages = 3;
+template <int D> constexpr int q_lds_bytes() { return kQStages * kv_unit_frags<D>() * 1024; }
 
 // ---------------------------------------------------------------- dK, dV
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void attention_backward_kv_kernel(BackwardArgs a) {
+__device__ __forceinline__ void backward_kv(const BackwardArgs& a, int index, lds_char* lds, float (*scratch)[kWaves]) {
     typedef typename Elem<T>::vec8 vec8;
     constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = q_unit_frags<D>(), S = stages<D>(), R = D > 128 && D < 256 ? 8 : 4;
     constexpr int kBytes = FRAGS * 1024;
-    __shared__ __attribute__((aligned(1024))) char lds_buf[S * kBytes];
-    lds_char* const lds = (lds_char*)lds_buf;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const TileWork work = tile_work(a.kv_tiles);
+    const TileWork work = tile_work(a.kv_tiles, index);
     const int bh = work.tile / a.kv_tiles.per_head;
     const int tile = work.tile - bh * a.kv_tiles.per_head;
     const int batch = bh / a.k.heads;
@@ -445,8 +454,7 @@ void attention_backward_kv_kernel(BackwardArgs a) {
         if constexpr (S == 3) copy_unit<FRAGS>(unit_of(i0 + 1), base + kBytes, wave, lane * 16);
     }
     constexpr int NV = kValuesInLds<D> ? N - 1 : N;
-    __shared__ __attribute__((aligned(1024))) char own_buf[kValuesInLds<D> ? kWaves * KT * 1024 : 16];
-    lds_char* const own_v = (lds_char*)own_buf + (kValuesInLds<D> ? wave * KT * 1024 + lane * 16 : 0);
+    lds_char* const own_v = lds + S * kBytes + wave * KT * 1024 + lane * 16;
     vec8 kf[N][KT], vf[NV][KT];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -466,7 +474,7 @@ void attention_backward_kv_kernel(BackwardArgs a) {
     if constexpr (kScaled<T>) {
         const int q_blocks = a.kv_group * (a.q_units / 2), kv_blocks = a.kv_units / 2;
         e = shift_of(bound_of(a.q_most + (int64_t)bh * q_blocks, q_blocks, a.v_most + (int64_t)bh * kv_blocks, kv_blocks,
-                              a.l_most + (int64_t)bh * q_blocks));
+                              a.l_most + (int64_t)bh * q_blocks, scratch));
     }
     const float f = __builtin_amdgcn_exp2f(e - kShift16);
     f32x16 dk[N][MD], dv[N][MD];
@@ -571,7 +579,7 @@ void attention_backward_kv_kernel(BackwardArgs a) {
         const bool inside = key < a.kv_tokens, live = key < length;
         const int64_t at = inside ? key : 0;
         float* slot = nullptr;
-        if (work.slot >= 0) slot = a.part + (((int64_t)work.slot * kWaves + wave) * N + n) * MD * 1024;
+        if (work.slot >= 0) slot = a.kv_part + (((int64_t)work.slot * kWaves + wave) * N + n) * MD * 1024;
         store_unit<T, MD>(dk[n], kfac, live, slot, reinterpret_cast<T*>(a.dk.data) + a.dk.row(bh, at), inside, a.head_dim, lane);
         if (slot) slot += (int64_t)a.kv_tiles.parts * a.kv_tiles.rest * kWaves * N * MD * 1024;
         store_unit<T, MD>(dv[n], vfac, live, slot, reinterpret_cast<T*>(a.dv.data) + a.dv.row(bh, at), inside, a.head_dim, lane);
@@ -580,16 +588,13 @@ void attention_backward_kv_kernel(BackwardArgs a) {
 
 // ---------------------------------------------------------------- dQ
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void attention_backward_q_kernel(BackwardArgs a) {
+__device__ __forceinline__ void backward_q(const BackwardArgs& a, int index, lds_char* lds, float (*scratch)[kWaves]) {
     typedef typename Elem<T>::vec8 vec8;
-    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kv_unit_frags<D>(), S = 3, R = D <= 128 ? 6 : D == 160 ? 10 : 12;
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kv_unit_frags<D>(), S = kQStages, R = D <= 128 ? 6 : D == 160 ? 10 : 12;
     constexpr int kBytes = FRAGS * 1024;
-    __shared__ __attribute__((aligned(1024))) char lds_buf[S * kBytes];
-    lds_char* const lds = (lds_char*)lds_buf;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const TileWork work = tile_work(a.q_tiles);
+    const TileWork work = tile_work(a.q_tiles, index);
     const int bh = work.tile / a.q_tiles.per_head;
     const int tile = work.tile - bh * a.q_tiles.per_head;
     const int kv_bh = bh / a.kv_group;
@@ -629,7 +634,7 @@ void attention_backward_q_kernel(BackwardArgs a) {
     if constexpr (kScaled<T>) {
         const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
         e = shift_of(bound_of(a.q_most + (int64_t)bh * q_blocks, q_blocks, a.v_most + (int64_t)kv_bh * kv_blocks, kv_blocks,
-                              a.l_most + (int64_t)bh * q_blocks));
+                              a.l_most + (int64_t)bh * q_blocks, scratch));
 #pragma unroll
         for (int n = 0; n < N; ++n) nl[n] += e - kShift16;
     }
@@ -729,10 +734,25 @@ void attention_backward_q_kernel(BackwardArgs a) {
         const int row = unit * kUnit + col;
         const bool inside = row < a.q_tokens;
         float* slot = nullptr;
-        if (work.slot >= 0) slot = a.part + (((int64_t)work.slot * kWaves + wave) * N + n) * MD * 1024;
+        if (work.slot >= 0) slot = a.q_part + (((int64_t)work.slot * kWaves + wave) * N + n) * MD * 1024;
         store_unit<T, MD>(dq[n], fac, true, slot, reinterpret_cast<T*>(a.dq.data) + a.dq.row(bh, inside ? row : 0), inside,
                           a.head_dim, lane);
     }
+}
+
+// Workgroups [0, kv): tiles of dK and dV; the rest: tiles of dQ.  One launch, so
+// that CUs that have no tile of the first left go on with the second.
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void attention_backward_kernel(BackwardArgs a) {
+    constexpr int kBytes = kv_lds_bytes<D>() > q_lds_bytes<D>() ? kv_lds_bytes<D>() : q_lds_bytes<D>();
+    __shared__ __attribute__((aligned(1024))) char lds[kBytes];
+    __shared__ float scratch[3][kWaves];
+    const int kv = a.kv_tiles.whole + a.kv_tiles.rest * a.kv_tiles.parts;
+    if ((int)blockIdx.x < kv)
+        backward_kv<T, D>(a, blockIdx.x, (lds_char*)lds, scratch);
+    else
+        backward_q<T, D>(a, blockIdx.x - kv, (lds_char*)lds, scratch);
 }
 
 template <typename T, int D>
@@ -743,23 +763,14 @@ int launch_t(const BackwardArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((attention_backward_pack_kernel<T, D>), dim3(bh * a.q_units + kv_bh * a.kv_units), dim3(256),
                        0, stream, a);
     if ((rc = pisa_host::check_launch("attention_backward_pack_kernel"))) return rc;
-    auto workgroups = [](const BackwardTiles& p) { return dim3(p.whole + p.rest * p.parts); };
-    auto join = [&](const BackwardTiles& p, int tensors, int units, int tokens, const OutView& out0, const OutView& out1) {
-        if (p.parts <= 1) return PISA_OK;
-        hipLaunchKernelGGL((attention_backward_join_kernel<T, MD, kTile>), dim3(tensors * p.rest * kTile * MD), dim3(64), 0,
-                           stream, a.part, p, units, tokens, a.head_dim, out0, out1);
-        return pisa_host::check_launch("attention_backward_join_kernel");
-    };
-    if (a.dk.data) {
-        hipLaunchKernelGGL((attention_backward_kv_kernel<T, D>), workgroups(a.kv_tiles), dim3(64 * kWaves), 0, stream, a);
-        if ((rc = pisa_host::check_launch("attention_backward_kv_kernel")) ||
-            (rc = join(a.kv_tiles, 2, a.kv_units, a.kv_tokens, a.dk, a.dv)))
-            return rc;
-    }
-    if (!a.dq.data) return PISA_OK;
-    hipLaunchKernelGGL((attention_backward_q_kernel<T, D>), workgroups(a.q_tiles), dim3(64 * kWaves), 0, stream, a);
-    if ((rc = pisa_host::check_launch("attention_backward_q_kernel"))) return rc;
-    return join(a.q_tiles, 1, a.q_units, a.q_tokens, a.dq, a.dq);
+    auto workgroups = [](const BackwardTiles& p) { return p.whole + p.rest * p.parts; };
+    hipLaunchKernelGGL((attention_backward_kernel<T, D>), dim3(workgroups(a.kv_tiles) + workgroups(a.q_tiles)),
+                       dim3(64 * kWaves), 0, stream, a);
+    if ((rc = pisa_host::check_launch("attention_backward_kernel"))) return rc;
+    const int joined = (a.kv_tiles.parts > 1 ? 2 * a.kv_tiles.rest : 0) + (a.q_tiles.parts > 1 ? a.q_tiles.rest : 0);
+    if (joined == 0) return PISA_OK;
+    hipLaunchKernelGGL((attention_backward_join_kernel<T, MD, kTile>), dim3(joined * kTile * MD), dim3(64), 0, stream, a);
+    return pisa_host::check_launch("attention_backward_join_kernel");
 }
 
 template <typename T>
@@ -777,39 +788,110 @@ int launch_d(int padded, const BackwardArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// A tile's workgroup has a CU to itself, so the tiles run in rounds of 256.  Those
-// of the last, partial round (all of them in a small problem) are split over as
-// many workgroups as fill the CUs, while each part keeps eight units.
-static BackwardTiles split_tiles(int64_t heads, int units, int units_per_tile, int64_t steps) {
-    constexpr int kSlots = 256;
+// ---- how the tiles are split
+// A tile's workgroup has a CU to itself.  The tiles of dK and dV are dispatched
+// first, those of dQ as CUs become free.  Splitting the streamed side of every
+// tile of a kind over several workgroups shortens the end of a launch and fills
+// CUs that a small problem leaves idle; it costs a start-up and an fp32 write for
+// each part and the launch that joins them.  plan_tiles takes the numbers of
+// parts with the smallest estimate of the launch's end.  Costs are in quarters
+// of the time of a dK, dV step at width 128 (about 0.45 us).
+struct TileKind {
+    int64_t tiles;  // 0: not formed
+    int64_t steps;
+    double step_cost, tile_bytes;
+};
+
+constexpr int kSlots = 256;        // workgroups at once
+constexpr double kStart = 16.0;    // start-up and end of a workgroup
+constexpr double kJoin = 18.0;     // the joining launch
+constexpr double kByteCost = 1.0 / 2.25e6;
+
+// End of a launch of m0 workgroups of cost c0 followed by m1 of cost c1, each
+// taken by the slot that is free first.
+static double end_of(int64_t m0, double c0, int64_t m1, double c1) {
+    const int64_t rounds = m0 / kSlots, late = m0 % kSlots;  // `late` slots are free a c0 after the others
+    const double t0 = rounds * c0, t1 = t0 + (late ? c0 : 0.0);
+    if (m1 == 0) return t1;
+    const int64_t early = kSlots - late;
+    auto done = [&](double t) {  // of the second kind by time t
+        return early * static_cast<int64_t>((t - t0) / c1 + 1e-9) +
+               (t > t1 ? late * static_cast<int64_t>((t - t1) / c1 + 1e-9) : 0);
+    };
+    // the end is a multiple of c1 after t0 or t1: just below and above the even share
+    const double even = (m1 * c1 + early * t0 + late * t1) / kSlots;
+    double best = 1e300;
+    for (int g = 0; g < 2; ++g) {
+        const double from = g == 0 ? t0 : t1;
+        int64_t k = static_cast<int64_t>((even - from) / c1);
+        if (k < 0) k = 0;
+        for (int64_t i = k; i < k + 3; ++i)
+            if (done(from + i * c1) >= m1) {
+                if (from + i * c1 < best) best = from + i * c1;
+                break;
+            }
+    }
+    return best > t1 ? best : t1;
+}
+
+static void plan_tiles(const TileKind& kv, const TileKind& q, int& kv_parts, int& q_parts) {
+    constexpr int kMostParts = 32;
+    auto most = [](const TileKind& x) {
+        const int64_t n = x.tiles >= 4 * kSlots ? 1 : x.steps / 8;  // eight steps to a part at least
+        return static_cast<int>(n < 1 ? 1 : n > kMostParts ? kMostParts : n);
+    };
+    double best = 1e300;
+    kv_parts = q_parts = 1;
+    const int kv_most = kv.tiles ? most(kv) : 1, q_most = q.tiles ? most(q) : 1;
+    for (int i = 1; i <= kv_most; ++i)
+        for (int j = 1; j <= q_most; ++j) {
+            const double kv_cost = (kv.steps + i - 1) / i * kv.step_cost + kStart;
+            const double q_cost = (q.steps + j - 1) / j * q.step_cost + kStart;
+            double cost = end_of(kv.tiles * i, kv_cost, q.tiles * j, q_cost);
+            if ((kv.tiles && i > 1) || (q.tiles && j > 1)) cost += kJoin;
+            // parts are written and read again
+            if (i > 1) cost += 2.0 * kv.tiles * i * kv.tile_bytes * kByteCost;
+            if (j > 1) cost += 2.0 * q.tiles * j * q.tile_bytes * kByteCost;
+            if (cost < best) {
+                best = cost;
+                kv_parts = i;
+                q_parts = j;
+            }
+        }
+}
+
+static BackwardTiles tiles_of(const TileKind& x, int per_head, int parts) {
     BackwardTiles p;
-    p.per_head = (units + units_per_tile - 1) / units_per_tile;
-    const int64_t tiles = heads * p.per_head;
-    p.whole = static_cast<int>(tiles / kSlots * kSlots);
-    p.rest = static_cast<int>(tiles - p.whole);
-    int64_t parts = p.rest > 0 ? kSlots / p.rest : 1;
-    if (parts > steps / 8) parts = steps / 8;
-    p.parts = parts < 1 ? 1 : static_cast<int>(parts);
+    p.per_head = per_head;
+    p.whole = parts > 1 ? 0 : static_cast<int>(x.tiles);
+    p.rest = parts > 1 ? static_cast<int>(x.tiles) : 0;
+    p.parts = parts;
     return p;
 }
 
-BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int padded, bool scaled) {
+BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int padded, bool scaled,
+                           bool with_q, bool with_kv) {
     BackwardPlan p;
     const int tile = kWaves * (padded <= 128 ? 2 : 1);
     p.q_units = (q_tokens + kBlock - 1) / kBlock * 2;
     p.kv_units = (kv_tokens + kBlock - 1) / kBlock * 2;
     const int64_t bh = (int64_t)batch * heads, kv_bh = (int64_t)batch * kv_heads;
-    p.q_tiles = split_tiles(bh, p.q_units, tile, p.kv_units);
-    p.kv_tiles = split_tiles(kv_bh, p.kv_units, tile, (int64_t)p.q_units * (heads / kv_heads));
+    const int q_per_head = (p.q_units + tile - 1) / tile, kv_per_head = (p.kv_units + tile - 1) / tile;
+    const double tile_bytes = (double)tile * padded * kUnit * sizeof(float), width = padded / 128.0 * (padded <= 128 ? 1 : 0.6);
+    const TileKind kv{with_kv ? kv_bh * kv_per_head : 0, (int64_t)p.q_units * (heads / kv_heads), 4 * width, 2 * tile_bytes};
+    const TileKind q{with_q ? bh * q_per_head : 0, p.kv_units, 3 * width, tile_bytes};
+    int kv_parts, q_parts;
+    plan_tiles(kv, q, kv_parts, q_parts);
+    p.kv_tiles = tiles_of(kv, kv_per_head, kv_parts);
+    p.q_tiles = tiles_of(q, q_per_head, q_parts);
     p.qx_bytes = bh * p.q_units * (4 * (padded / 16) + 1) * 1024;
     p.kx_bytes = kv_bh * p.kv_units * 3 * (padded / 16) * 1024;
     p.q_most_bytes = scaled ? bh * (p.q_units / 2) * (int64_t)sizeof(float) : 0;
     p.l_most_bytes = p.q_most_bytes;
     p.v_most_bytes = scaled ? kv_bh * (p.kv_units / 2) * (int64_t)sizeof(float) : 0;
-    const int64_t tile_bytes = (int64_t)tile * padded * kUnit * sizeof(float);
-    const int64_t q_part = p.q_tiles.parts > 1 ? p.q_tiles.parts * p.q_tiles.rest * tile_bytes : 0;
-    const int64_t kv_part = p.kv_tiles.parts > 1 ? 2 * p.kv_tiles.parts * p.kv_tiles.rest * tile_bytes : 0;
-    p.part_bytes = q_part > kv_part ? q_part : kv_part;  // the two kernels run one after the other
+    const int64_t part_bytes = (int64_t)tile * padded * kUnit * sizeof(float);
+    p.q_part_bytes = q_parts > 1 ? q_parts * q.tiles * part_bytes : 0;
+    p.kv_part_bytes = kv_parts > 1 ? 2 * kv_parts * kv.tiles * part_bytes : 0;
     return p;
 }
 

@@ -311,7 +311,7 @@ struct BackwardArgs {
     char *qx, *kx;              // packed units
     // largest row norms of dO and V and largest |dlse| by 64-row block (fp16): [BH][q_units/2], [BHk][kv_units/2]
     float *q_most, *v_most, *l_most;
-    float* part;                // fp32 gradients of the parts
+    float *q_part, *kv_part;    // fp32 gradients of the parts
     __device__ __forceinline__ int length(int b) const {
         return kv_lengths ? min(max(kv_lengths[b], 0), kv_tokens) : kv_tokens;
     }
@@ -319,9 +319,10 @@ struct BackwardArgs {
 struct BackwardPlan {
     int q_units, kv_units;
     BackwardTiles q_tiles, kv_tiles;
-    int64_t qx_bytes, kx_bytes, q_most_bytes, v_most_bytes, l_most_bytes, part_bytes;
+    int64_t qx_bytes, kx_bytes, q_most_bytes, v_most_bytes, l_most_bytes, q_part_bytes, kv_part_bytes;
 };
-BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int padded, bool scaled);
+BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int padded, bool scaled,
+                           bool with_q, bool with_kv);
 int launch_attention_backward(int dtype, int padded, const BackwardArgs& a, hipStream_t stream);
 
 }  // namespace pisa
