@@ -1008,7 +1008,7 @@ int launch_attention_t(const ArgsFor<TRAIN>& a_in, int bh_count, hipStream_t str
 // attention_train.hip: the dense kernels' training variant, under the same scheduler.
 // Work items that leave SIMDs idle are shared by two or four waves each, where the
 // rounds of the SIMDs times a wave's chunks (and about four chunks' time for a
-// merge) come out smaller: [1,8,1000,64] 19.2 -> 10.5 us with four.  (Fuller grids
+// merge) come out smaller.  (Fuller grids
 // stay as they are: [2,16,9216,128] 1270-1300 us, 1304 with two.)
 template <typename T, int D>
 static int launch_train_d(const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
@@ -1031,7 +1031,6 @@ static int launch_train_d(const AttnTrainArgs& a, int bh_count, hipStream_t stre
 template <typename T>
 static int launch_train_t(int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
     switch (padded) {
-        case 64: return launch_train_d<T, 64>(a, bh_count, stream);
         case 96: return launch_train_d<T, 96>(a, bh_count, stream);
         case 128: return launch_train_d<T, 128>(a, bh_count, stream);
         case 160: return launch_train_d<T, 160>(a, bh_count, stream);
@@ -1041,6 +1040,7 @@ static int launch_train_t(int padded, const AttnTrainArgs& a, int bh_count, hipS
     }
 }
 int launch_attention_train(int dtype, int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
+    if (padded == 64) return launch_attention_d64_train(dtype, a, bh_count, stream);
     if (dtype == PISA_DTYPE_BF16) return launch_train_t<bf16_t>(padded, a, bh_count, stream);
     return launch_train_t<f16_t>(padded, a, bh_count, stream);
 }

@@ -4,6 +4,8 @@
 // (attention.hip describes the computation; the operand tables, the transposed
 // scores and the lazy softmax are the same; it also runs the dense packed calls
 // that give each SIMD at most one wave, dense_d64_one_wave).
+#include <type_traits>
+
 #include "attention_softmax.hpp"
 #include "kernels.hpp"
 
@@ -41,11 +43,17 @@ constexpr int kRawFlags = 0x00020000;  // untyped 32-bit buffer data format
 // width 64 20 instead of 8 per half: 4 of keys, from 32 rows each, and 16 of
 // values, from two rows each): dense_rows_in_place says when that is the better
 // trade.  Width 128 exists in this form only (340 registers, one wave per SIMD).
-template <typename T, int D, bool SPARSE, bool TAIL, int W, bool DIRECT>
+//
+// TRAIN (dense, packed): grouped key heads, a key count per batch entry and the
+// rows' log sums as an output, as in attention.hip.
+template <bool TRAIN> using ArgsFor = std::conditional_t<TRAIN, AttnTrainArgs, AttnArgs>;
+
+template <typename T, int D, bool SPARSE, bool TAIL, int W, bool DIRECT, bool TRAIN = false>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 2 : 1, D <= 64 ? 2 : 1)))
-void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ sel,
+void attention_parts_kernel(ArgsFor<TRAIN> a, KvRows kv, const int32_t* __restrict__ sel,
                             const uint32_t* __restrict__ selmask) {
     static_assert(!DIRECT || (!SPARSE && !TAIL), "rows are read in place by the dense kernel only");
+    static_assert(!TRAIN || (!SPARSE && !TAIL && !DIRECT), "the training forward is dense and packed");
     static_assert(D == 64 || (D == 128 && DIRECT), "packed tables of other widths: attention.hip");
     constexpr int KT = D / 16;  // 16-deep k-steps of the score products
     constexpr int MD = D / 32;  // 32-dim output tiles
@@ -101,10 +109,22 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
 
     // ---- chunk list: [0, n_exact) exact blocks, [n_exact, n_chunks) centroid
     // chunks; this wave's part is [lo, hi), never empty (W <= n_chunks)
-    const int n_exact = SPARSE ? a.exact : a.kv_blocks;
+    // except with TRAIN and fewer keys than the tables hold
+    int kv_tokens = a.kv_tokens, kv_bh = bh;
+    if constexpr (TRAIN) {
+        kv_bh = bh / a.kv_group;
+        if (a.kv_lengths) kv_tokens = min(max(a.kv_lengths[bh / a.q.heads], 0), kv_tokens);
+    }
+    const int n_exact = SPARSE ? a.exact : TRAIN ? (kv_tokens + kBlock - 1) / kBlock : a.kv_blocks;
     const int n_chunks = n_exact + (TAIL ? a.npad / kBlock : 0);
-    const int lo = wave * n_chunks / W;
-    const int hi = (wave + 1) * n_chunks / W;
+    int lo = wave * n_chunks / W;
+    int hi = (wave + 1) * n_chunks / W;
+    if constexpr (TRAIN) {
+        if (lo >= hi) {  // no chunk for this wave: one without a live key, which adds nothing (the table has one then)
+            lo = n_chunks;
+            hi = lo + 1;
+        }
+    }
     const int32_t* my_idx = SPARSE ? sel + ((int64_t)bh * a.q_blocks + qb) * a.exact : nullptr;
     const uint32_t* my_mask = TAIL ? selmask + ((int64_t)bh * a.q_blocks + qb) * a.mask_words : nullptr;
     // Packed tables of this head as buffer resources (reads past a table return
@@ -113,8 +133,8 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
     // through private memory, with a wait for every load in flight.
     const int tab_bytes = a.kv_blocks * kBlockBytes;
     const int cen_bytes = TAIL ? a.npad * D * 2 : 0;
-    const char* const kp = a.kp + (int64_t)bh * tab_bytes;
-    const char* const vp = a.vp + (int64_t)bh * tab_bytes;
+    const char* const kp = a.kp + (int64_t)kv_bh * tab_bytes;
+    const char* const vp = a.vp + (int64_t)kv_bh * tab_bytes;
     const char* const kc = TAIL ? a.kbar + (int64_t)bh * cen_bytes : kp;
     const char* const vc = TAIL ? a.vbar_t + (int64_t)bh * cen_bytes : vp;
     auto table = [&](bool tail, const char* exact, const char* centroids) {
@@ -137,7 +157,7 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
 
     auto is_tail = [&](int x) { return TAIL && min(x, n_chunks - 1) >= n_exact; };
     auto table_row = [&](int x) -> int {  // block id, or centroid chunk id; past the list, its last chunk again
-        x = min(x, n_chunks - 1);
+        x = min(x, (TRAIN ? a.kv_blocks : n_chunks) - 1);
         if (TAIL && x >= n_exact) return x - n_exact;
         return SPARSE ? my_idx[x] : x;
     };
@@ -260,10 +280,10 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
     // column maxima and running-max update of half mt of a chunk; `plain`: an
     // exact full block, else a short last key block is masked first
     auto check = [&](f32x16 (&s)[NT], bool tail, int row, int mt, bool plain) {
-        if (!plain && !tail && (row + 1) * kBlock > a.kv_tokens) {
+        if (!plain && !tail && (row + 1) * kBlock > kv_tokens) {
 #pragma unroll
             for (int v = 0; v < 16; ++v)
-                if (row * kBlock + mt * 32 + 8 * (v >> 2) + 4 * half + (v & 3) >= a.kv_tokens)
+                if (row * kBlock + mt * 32 + 8 * (v >> 2) + 4 * half + (v & 3) >= kv_tokens)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) s[nt][v] = -__builtin_inff();
         }
@@ -289,7 +309,7 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
         vec8 pf[NT][2];
         if (!half0_only) scores(sb, t0, row0, 1);
         if (!last) load_k(t1, row1, 0);
-        probs_half<T, NT>(sa, c, nm, l, lt, t0, pf);
+        probs_half<T, NT, TRAIN>(sa, c, nm, l, lt, t0, pf);
         pv(pf);
         if (!half0_only) {
             load_v(t0, row0, 1);
@@ -301,7 +321,7 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
             load_k(t1, row1, 1);
         }
         if (!half0_only) {
-            probs_half<T, NT>(sb, c, nm, l, lt, t0, pf);
+            probs_half<T, NT, TRAIN>(sb, c, nm, l, lt, t0, pf);
             pv(pf);
         }
         if (!last) {
@@ -357,6 +377,7 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
                 lt[nt] += stat[w][2][32 * nt + col] * f;
             }
             const float f = factor(m[nt]);
+            if constexpr (TRAIN) nm[nt] = -top;
 #pragma unroll
             for (int md = 0; md < MD; ++md)
 #pragma unroll
@@ -368,6 +389,15 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
                 }
         }
         __syncthreads();
+    }
+    if constexpr (TRAIN) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int tok = qbase + q_off[nt];
+            if (wave == 0 && half == 0 && tok < a.q_tokens)
+                a.lse[(int64_t)bh * a.q_tokens + tok] =
+                    n_chunks == 0 ? -__builtin_inff() : (__builtin_log2f(l[nt]) - nm[nt]) * kLn2;
+        }
     }
     const bool first_order = TAIL && a.ht != nullptr;
     const __amdgpu_buffer_rsrc_t ht_rs = __builtin_amdgcn_make_buffer_rsrc(
@@ -417,7 +447,7 @@ void attention_parts_kernel(AttnArgs a, KvRows kv, const int32_t* __restrict__ s
             for (int e = 0; e < 8; ++e) x[e] = o[u >> 2][(u >> 1) & 1][8 * (u & 1) + e];
         }
         const float lf = second ? l[1] : l[0];
-        const float inv = 1.0f / lf;
+        const float inv = TRAIN && n_chunks == 0 ? 0.0f : 1.0f / lf;
 #pragma unroll
         for (int e = 0; e < kVals; ++e) x[e] *= inv;
         if (first_order) {
@@ -524,14 +554,14 @@ int waves_per_block(int64_t blocks, int n_chunks, int most) {
     return best;
 }
 
-template <typename T, int D, bool SPARSE, bool TAIL, bool DIRECT>
-int launch_t(const AttnArgs& a, const KvRows& kv, int bh_count, hipStream_t stream) {
+template <typename T, int D, bool SPARSE, bool TAIL, bool DIRECT, bool TRAIN = false>
+int launch_t(const ArgsFor<TRAIN>& a, const KvRows& kv, int bh_count, hipStream_t stream) {
     const int blocks = bh_count * a.q_blocks;
     const int n_chunks = (SPARSE ? a.exact : a.kv_blocks) + (TAIL ? a.npad / kBlock : 0);
     constexpr int kMost = D <= 64 ? 8 : 4;  // waves of a workgroup: two per SIMD, one at D = 128
     const int w = waves_per_block(blocks, n_chunks, kMost);
 #define PISA_PARTS(W)                                                                                              \
-    hipLaunchKernelGGL((attention_parts_kernel<T, D, SPARSE, TAIL, W, DIRECT>), dim3(blocks), dim3(64 * W), 0, stream, \
+    hipLaunchKernelGGL((attention_parts_kernel<T, D, SPARSE, TAIL, W, DIRECT, TRAIN>), dim3(blocks), dim3(64 * W), 0, stream, \
                        a, kv, a.idx, a.selmask)
     if (w == 1) PISA_PARTS(1);
     else if (w == 2) PISA_PARTS(2);
@@ -554,6 +584,12 @@ int launch_t(const AttnArgs& a, const KvRows& kv, int bh_count, hipStream_t stre
 bool dense_d64_one_wave(const AttnArgs& a, int bh_count) {
     const int64_t blocks = (int64_t)bh_count * a.q_blocks;
     return blocks <= simd_count() && waves_per_block(blocks, a.kv_blocks, 8) == 1;
+}
+
+int launch_attention_d64_train(int dtype, const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
+    const KvRows none{};
+    return dtype == PISA_DTYPE_BF16 ? launch_t<bf16_t, 64, false, false, false, true>(a, none, bh_count, stream)
+                                    : launch_t<f16_t, 64, false, false, false, true>(a, none, bh_count, stream);
 }
 
 int launch_attention_d64(int dtype, bool sparse, const AttnArgs& a, int bh_count, hipStream_t stream) {
