@@ -42,35 +42,40 @@ def rope_frequencies(axes_dims: Sequence[int], theta: float | Sequence[float] = 
 
 
 # --------------------------------------------------------------------------- checks
-def _check_rows(what: str, name: str, x, like=None, dtype=None) -> None:
+def _check_rows(what: str, name: str, x, like=None) -> None:
+    """Every attribute is read once: these checks bound small calls."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: {name} must be a torch tensor.")
-    if x.ndim != 4 or min(x.shape) <= 0:
-        raise ValueError(f"{what}: {name} must be [B,H,T,D] with every dimension positive, got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 4 or 0 in shape:
+        raise ValueError(f"{what}: {name} must be [B,H,T,D] with every dimension positive, got {tuple(shape)}")
     if not _is_rocm_device(x):
         raise ValueError(f"{what}: {name} must be on a PyTorch ROCm device.")
     if x.dtype not in ROPE_DTYPES:
         raise ValueError(f"{what}: {name} must be bfloat16, float16 or float32, got {x.dtype}")
-    if x.shape[3] not in ROPE_HEAD_DIMS:
-        raise ValueError(f"{what}: head dim must be a multiple of 8 up to 256, got {x.shape[3]}")
-    if x.shape[3] > 1 and x.stride(3) != 1:
+    if shape[3] % 8 or shape[3] > 256:
+        raise ValueError(f"{what}: head dim must be a multiple of 8 up to 256, got {shape[3]}")
+    if x.stride(3) != 1:
         raise ValueError(f"{what}: {name}'s head_dim must have unit stride")
     if like is not None:
-        if x.shape[0] != like.shape[0] or x.shape[2:] != like.shape[2:]:
-            raise ValueError(f"{what}: {name} {tuple(x.shape)} must share batch, tokens and head dim with "
-                             f"{tuple(like.shape)}")
+        other = like.shape
+        if shape[0] != other[0] or shape[2] != other[2] or shape[3] != other[3]:
+            raise ValueError(f"{what}: {name} {tuple(shape)} must share batch, tokens and head dim with {tuple(other)}")
         if x.device != like.device or x.dtype != like.dtype:
             raise ValueError(f"{what}: {name} must share q's device and dtype")
 
 
 def _check_weights(what: str, q, weights) -> None:
-    given = [w for w in weights if w is not None]
-    for w in given:
+    first = None
+    for w in weights:
+        if w is None:
+            continue
         if not isinstance(w, torch.Tensor):
             raise TypeError(f"{what}: weights must be torch tensors.")
-        if tuple(w.shape) != (q.shape[3],) or w.device != q.device or not w.is_contiguous():
+        if w.ndim != 1 or w.shape[0] != q.shape[3] or w.device != q.device or not w.is_contiguous():
             raise ValueError(f"{what}: a weight must be contiguous [{q.shape[3]}] on q's device, got {tuple(w.shape)}")
-        if w.dtype not in (q.dtype, torch.float32) or w.dtype != given[0].dtype:
+        first = w.dtype if first is None else first
+        if w.dtype != first or (first != torch.float32 and first != q.dtype):
             raise ValueError(f"{what}: weights must share one dtype, q's or float32, got {w.dtype}")
 
 
@@ -89,9 +94,9 @@ def _check_rotation(what: str, x, inv_freq, axes_dims, positions, token_grid) ->
         return ()
     if axes_dims is None or not 1 <= len(axes_dims) <= ROPE_MAX_AXES:
         raise ValueError(f"{what}: axes_dims must name 1 to {ROPE_MAX_AXES} axes")
-    axes = tuple(int(d) for d in axes_dims)
+    axes = tuple([int(d) for d in axes_dims])
     rotated = sum(axes)
-    if any(d <= 0 or d % 2 for d in axes) or rotated % 8 or rotated > x.shape[3]:
+    if rotated % 8 or rotated > x.shape[3] or min(axes) <= 0 or any([d % 2 for d in axes]):
         raise ValueError(f"{what}: axes_dims {axes} must be positive even numbers whose sum is a multiple of 8 and at "
                          f"most the head dim {x.shape[3]}")
     if not isinstance(inv_freq, torch.Tensor):
@@ -113,7 +118,8 @@ def _check_rotation(what: str, x, inv_freq, axes_dims, positions, token_grid) ->
         raise TypeError(f"{what}: positions must be a torch tensor.")
     if positions.dtype not in _POSITION_KINDS or positions.device != x.device:
         raise ValueError(f"{what}: positions must be int32, int64 or float32 on the input's device")
-    if tuple(positions.shape) not in ((tokens, len(axes)), (1, tokens, len(axes)), (batch, tokens, len(axes))):
+    where = positions.shape
+    if where[-2:] != (tokens, len(axes)) or len(where) not in (2, 3) or (len(where) == 3 and where[0] not in (1, batch)):
         raise ValueError(f"{what}: positions must be [T,A] or [B,T,A] with T={tokens} and A={len(axes)}, got "
                          f"{tuple(positions.shape)}")
     if positions.requires_grad:
@@ -122,26 +128,28 @@ def _check_rotation(what: str, x, inv_freq, axes_dims, positions, token_grid) ->
 
 
 # --------------------------------------------------------------------------- launchers
+_DIMS = _lib.ctypes.c_int32 * ROPE_MAX_AXES
+_NO_GRID = _lib.grid()
+
+
 def _rope_struct(inv_freq, axes, positions, grid, interleaved: bool, inverse: bool) -> _lib.PisaRope:
-    r = _lib.PisaRope()
-    r.interleaved, r.inverse, r.axes = int(interleaved), int(inverse), len(axes)
     if not axes:
-        return r
-    r.inv_freq = inv_freq.data_ptr()
-    r.axis_dims = (*axes, *(0,) * (ROPE_MAX_AXES - len(axes)))
+        return _lib.PisaRope(None, None, 0, 0, 0, _NO_GRID, 0, 0, _DIMS(), interleaved, inverse)
+    dims = _DIMS(*axes)
     if positions is None:
-        r.positions_kind, r.grid = _lib.POSITIONS_GRID, _lib.grid(*grid)
-        return r
-    r.positions_kind, r.positions = _POSITION_KINDS[positions.dtype], positions.data_ptr()
-    r.batch_stride = positions.stride(0) if positions.ndim == 3 and positions.shape[0] > 1 else 0
-    r.token_stride, r.axis_stride = positions.stride(-2), positions.stride(-1)
-    return r
+        return _lib.PisaRope(inv_freq.data_ptr(), None, 0, 0, 0, _lib.grid(*grid), _lib.POSITIONS_GRID, len(axes), dims,
+                             interleaved, inverse)
+    strides = positions.stride()
+    batch = strides[0] if len(strides) == 3 and positions.shape[0] > 1 else 0
+    return _lib.PisaRope(inv_freq.data_ptr(), positions.data_ptr(), batch, strides[-2], strides[-1], _NO_GRID,
+                         _POSITION_KINDS[positions.dtype], len(axes), dims, interleaved, inverse)
 
 
 def _heads_last(x) -> torch.Tensor:
     """An empty [B,H,T,D] view of contiguous [B,T,H,D] storage, the layout that the attention calls read best."""
     batch, heads, tokens, dim = x.shape
-    return x.new_empty((batch, tokens, heads, dim)).permute(0, 2, 1, 3)
+    return torch.empty_strided((batch, heads, tokens, dim), (tokens * heads * dim, dim, heads * dim, 1), dtype=x.dtype,
+                               device=x.device)
 
 
 def _view(x) -> _lib.PisaView:
