@@ -317,3 +317,37 @@ def test_refusals_on_the_device(ops):
     g = torch.autograd.grad(ops.axial_rope(x, **good).square().sum(), x, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_in_place_through_the_c_abi(ops):
+    """The C entry point may write its outputs over q and k."""
+    from mi355x_pisa import _lib, rotary
+
+    shape, axes = (2, 5, 120, 128), (44, 42, 42)
+    turn, _ = _turn(ops, "grid", shape, axes)
+    q, k = (_rows(i, shape, BF16) for i in (1, 2))
+    w = torch.rand(128, device="cuda")
+    want = ops.qk_norm_rope(q, k, w, w, **turn)
+    rope = rotary._rope_struct(turn["inv_freq"], axes, None, turn["token_grid"], False, False)
+    vq, vk = _lib.view4(q), _lib.view4(k)
+    _lib.check(_lib.LIB.attn_hip_qk_norm_rope(0, 2, 2, 5, 5, 120, 128, vq, vk, vq, vk, w.data_ptr(), w.data_ptr(), 1, 1e-6,
+                                              rope, _lib.stream_of(q.device)), "in place")
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+@pytest.mark.parametrize("size", [1e-19, 1e-3, 1e18])
+def test_rows_of_any_size_without_eps(ops, size):
+    """eps = 0: the mean square of a row may lie near the ends of fp32's range (1e-38 here, where it has all its bits)."""
+    x = (torch.randn((1, 2, 7, 64), generator=torch.Generator().manual_seed(1)) * size).cuda()
+    _near(ops.qk_norm_rope(x, None, eps=0.0)[0], *norm_rope(x, None, 0.0, None, False), "y")
+
+
+def test_many_heads_and_batches(ops):
+    """Heads beyond what a tile of several tokens takes, and tiles that end inside a batch entry."""
+    for shape, k_heads in (((1, 5000, 3, 8), 7), ((3, 2, 9001, 8), 1)):
+        q, k = _rows(1, shape, F32), _rows(2, (shape[0], k_heads, *shape[2:]), F32)
+        pos = torch.arange(shape[2], device="cuda", dtype=torch.int32)[:, None]
+        turn = {"inv_freq": ops.rope_frequencies((8,), device="cuda"), "axes_dims": (8,), "positions": pos}
+        angle = angles(turn["inv_freq"], (8,), pos)
+        for x, y in zip((q, k), ops.qk_norm_rope(q, k, **turn)):
+            _near(y, *norm_rope(x, None, 1e-6, angle, False), str(tuple(x.shape)))
