@@ -36,6 +36,7 @@
 // their bits to its small range: P is scaled by 2^15, and dS by a power of two
 // from the bound |dP - delta + dL| <= 2 max_i |dO_i| max_j |V_j| + max_i |dL_i| of the head, which
 // puts its largest possible value just under 2^15; the gradients are scaled back in fp32.
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -837,12 +838,14 @@ static double end_of(int64_t m0, double c0, int64_t m1, double c1) {
 static void plan_tiles(const TileKind& kv, const TileKind& q, int& kv_parts, int& q_parts) {
     constexpr int kMostParts = 32;
     auto most = [](const TileKind& x) {
-        const int64_t n = x.tiles >= 4 * kSlots ? 1 : x.steps / 8;  // eight steps to a part at least
+        if (x.tiles == 0 || x.tiles >= 4 * kSlots) return 1;
+        // eight steps to a part at least, and hardly more parts than fill the CUs
+        const int64_t n = std::min(x.steps / 8, (kSlots + x.tiles - 1) / x.tiles + 1);
         return static_cast<int>(n < 1 ? 1 : n > kMostParts ? kMostParts : n);
     };
     double best = 1e300;
     kv_parts = q_parts = 1;
-    const int kv_most = kv.tiles ? most(kv) : 1, q_most = q.tiles ? most(q) : 1;
+    const int kv_most = most(kv), q_most = most(q);
     for (int i = 1; i <= kv_most; ++i)
         for (int j = 1; j <= q_most; ++j) {
             const double kv_cost = (kv.steps + i - 1) / i * kv.step_cost + kStart;

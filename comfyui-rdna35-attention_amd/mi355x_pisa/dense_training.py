@@ -26,6 +26,7 @@ _NO_VIEW = _lib.PisaView(None, 0, 0, 0)
 
 # --------------------------------------------------------------------------- checks
 def _check_call(what: str, q, k, v, scale, kv_lengths) -> float:
+    """Every attribute is read once: these checks bound small calls."""
     if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
         raise TypeError(f"{what}: q, k, and v must be torch tensors.")
     qs, ks, vs = q.shape, k.shape, v.shape
@@ -35,20 +36,21 @@ def _check_call(what: str, q, k, v, scale, kv_lengths) -> float:
         raise ValueError(f"{what}: k {tuple(ks)} and v {tuple(vs)} must match")
     if qs[0] != ks[0] or qs[3] != ks[3]:
         raise ValueError(f"{what}: q {tuple(qs)} and k/v {tuple(ks)} must share batch and head dim")
-    if min(qs) <= 0 or min(ks) <= 0:
+    if 0 in qs or 0 in ks:
         raise ValueError(f"{what}: every dimension must be positive")
     if qs[1] % ks[1]:
         raise ValueError(f"{what}: {ks[1]} key heads do not divide {qs[1]} query heads")
-    if q.device != k.device or q.device != v.device or q.device.type != "cuda" or not _HIP:
+    device, dtype = q.device, q.dtype
+    if device != k.device or device != v.device or device.type != "cuda" or not _HIP:
         raise ValueError(f"{what}: q/k/v must be on one PyTorch ROCm device.")
-    if q.dtype not in TRAIN_DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"{what}: q/k/v must share one dtype of bfloat16/float16, got {q.dtype}/{k.dtype}/{v.dtype}")
+    if dtype not in TRAIN_DTYPES or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"{what}: q/k/v must share one dtype of bfloat16/float16, got {dtype}/{k.dtype}/{v.dtype}")
     if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1:
         raise ValueError(f"{what}: head_dim must have unit stride")
     if kv_lengths is not None:
         if not isinstance(kv_lengths, torch.Tensor):
             raise TypeError(f"{what}: kv_lengths must be a torch tensor.")
-        if kv_lengths.dtype != torch.int32 or tuple(kv_lengths.shape) != (qs[0],) or kv_lengths.device != q.device \
+        if kv_lengths.dtype != torch.int32 or tuple(kv_lengths.shape) != (qs[0],) or kv_lengths.device != device \
                 or not kv_lengths.is_contiguous():
             raise ValueError(f"{what}: kv_lengths must be contiguous int32 [{qs[0]}] on q's device")
     scale = float(scale)
