@@ -48,67 +48,82 @@ namespace {
 
 constexpr int kWaves = 4;       // waves of a workgroup, sharing the streamed units
 constexpr int kUnit = 32;       // streamed rows per step
+// Fragments read from LDS ahead of their use, a divisor of those of a unit (4 KT and 3 KT):
+// deeper rings measured the same, one of 3 in backward_kv up to 8 % slower.
+constexpr int kKvAhead = 4, kQAhead = 6;
 constexpr float kShift16 = 15;  // log2 of the factor on P in fp16
 
 template <typename T> constexpr bool kScaled = std::is_same<T, f16_t>::value;
 
-// Fragments of a unit, in the order in which they are used: query side [Q rows][dO rows][dO^T][Q^T] of D/16 KB each
-// and 1 KB of -L and dL - delta (32 floats each); key side [K rows][V rows][K^T].
-template <int D> constexpr int q_unit_frags() { return 4 * (D / 16) + 1; }
-template <int D> constexpr int kv_unit_frags() { return 3 * (D / 16); }
+// A unit is two operands of 32 rows (query side Q and dO, key side K and V) as
+// D/16 fragments of 1 KB, 16 dims of all rows each: the even ones, 128 bytes, the
+// odd ones.  The 128 bytes hold -L (beside Q) and dL - delta (beside dO) of the
+// rows, and put fragments 2m and 2m + 1 into different LDS banks.  Both forms of
+// an operand are read from it without bank conflicts: rows (A of the first
+// product) with one 16-byte read of a lane, columns (A of the second) with two
+// transposing 8-byte reads.
+template <int D> constexpr int kOperand = D * 64 + 128;  // bytes
+template <int D> constexpr int kGap = D * 32;            // of the 128 bytes between the even and the odd fragments
+template <int D> constexpr int kUnitFrags = D / 8 + 1;   // 1 KB pieces of a unit
+template <int D> constexpr int kUnitBytes = kUnitFrags<D> * 1024;
+// Byte in an operand of fragment t's lane 0, and of a lane in its fragment: dims 8 half .. of a row.
+template <int D> __host__ __device__ constexpr int frag_at(int t) { return t / 2 * 1024 + (t & 1) * (kGap<D> + 128); }
+__host__ __device__ constexpr int lane_at(int half, int row) { return half * 512 + (row ^ (4 * half)) * 16; }
+// What lane l points a transposing read at for dims 32 md .. and rows 16 s + 8 u +
+// 4 (l / 32) .., less md * 1024 + s * 256 + u * 128.  The 16 lanes of a group read
+// 4 rows of 16 dims; lane i of them receives dim i of the 4 rows.
+template <int D> __device__ __forceinline__ int transposing_at(int lane) {
+    const int j = lane & 15;
+    return frag_at<D>((lane >> 4) & 1) + lane_at((j >> 1) & 1, 4 * (lane >> 5) + (j >> 2)) + (j & 1) * 8;
+}
 
 // Columns per wave / 32.  Two use a fragment read from LDS twice; above 128 the
 // accumulators and own operands of 64 columns do not fit 512 registers.
 template <int D> constexpr int columns() { return D <= 128 ? 2 : 1; }
-template <int D> constexpr int stages() { return D <= 192 ? 3 : 2; }
 // At width 128 the values of a wave's second 32 keys stay in LDS (read again for
 // every unit): with them the kernel would need more than 512 registers.
 template <int D> constexpr bool kValuesInLds = D == 128;
 
 // ---------------------------------------------------------------- packing
-// One 64-row block of X into two units: 16-byte pieces of rows (fragment lane
-// (half, row) holds dims 16t + 8half ..) straight from registers, and the
-// transposed fragments (lane (half, dim) holds the rows at positions 16s +
-// 8half .. of swap23 order) through LDS.  Rows from `live` on and dims from d_real on
-// are zero.  With `dot`, red[0][row][piece] receives the pieces of sum_d X Y;
-// with `squares`, red[1][row][piece] those of sum_d X^2.
-template <typename T, int D> struct PackLds {
-    static constexpr int kPieces = D / 8;
-    T t[D * (kBlock + 8)];
-    float red[2][kBlock][kPieces + 1];
+// One 64-row block of X into an operand of two units, in 16-byte pieces: a wave
+// reads whole rows and writes runs of 16 bytes by its number of rows, which the
+// next rows' continue.  Rows from `live` on and dims from d_real on are zero.  With
+// y, red[0][row][piece] receives the pieces of sum_d X Y; with `squares`,
+// red[1][row][piece] those of sum_d X^2.
+template <int D> struct PackLds {
+    float red[2][kBlock][D / 8 + 1];
 };
 
 template <typename T, int D>
-__device__ __forceinline__ void pack_block(PackLds<T, D>& lds, const char* x, int64_t st, const char* y, int64_t yst,
-                                           int live, int last, int d_real, char* units, int64_t unit_bytes, int rows_at,
-                                           int trans_at, bool squares) {
+__device__ __forceinline__ void pack_block(PackLds<D>& lds, const char* x, int64_t st, const char* y, int64_t yst,
+                                           int live, int last, int d_real, char* units, bool squares) {
     typedef typename Elem<T>::vec8 vec8;
-    typedef T vec4 __attribute__((ext_vector_type(4)));
-    constexpr int kRow = kBlock + 8;
     constexpr int kPieces = D / 8;
     constexpr int kGroups = 256 / kPieces;
+    constexpr int kBatch = (kBlock + kGroups - 1) / kGroups;
     const int t = threadIdx.x;
     const int pc = t % kPieces;
     const int r0 = t / kPieces;
     const bool live_d = pc * 8 < d_real;
     const int dc = live_d ? pc * 8 : 0;
-    for (int r = r0 * 4; r0 < kGroups && r < kBlock; r += kGroups * 4) {
-        vec8 xv[4], yv[4];
+    if (r0 < kGroups) {
+        vec8 xv[kBatch], yv[kBatch];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // rows past the end read the last one
-            xv[i] = load8<vec8>(x + (min(r + i, last) * st + dc) * (int64_t)sizeof(T));
-            if (y) yv[i] = load8<vec8>(y + (min(r + i, last) * yst + dc) * (int64_t)sizeof(T));
+        for (int i = 0; i < kBatch; ++i) {  // rows past the end read the last one
+            const int r = min(r0 + i * kGroups, last);
+            xv[i] = load8<vec8>(x + (r * st + dc) * (int64_t)sizeof(T));
+            if (y) yv[i] = load8<vec8>(y + (r * yst + dc) * (int64_t)sizeof(T));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (r + i >= live || !live_d) {
+        for (int i = 0; i < kBatch; ++i) {
+            const int r = r0 + i * kGroups;
+            if (r >= kBlock) break;
+            if (r >= live || !live_d) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) xv[i][e] = T(0.0f);
                 if (y) yv[i] = xv[i];
             }
-            const int row = (r + i) & 31;
-            char* unit = units + ((r + i) >> 5) * unit_bytes;
-            if (rows_at >= 0) store8(unit + rows_at * 1024 + ((pc >> 1) * 64 + (pc & 1) * 32 + row) * 16, xv[i]);
+            store8(units + (r >> 5) * kUnitBytes<D> + frag_at<D>(pc >> 1) + lane_at(pc & 1, r & 31), xv[i]);
             float dot = 0.0f, sq = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -116,34 +131,15 @@ __device__ __forceinline__ void pack_block(PackLds<T, D>& lds, const char* x, in
                 if (y) dot = fmaf(f, to_f32(yv[i][e]), dot);
                 sq = fmaf(f, f, sq);
             }
-            if (y) lds.red[0][r + i][pc] = dot;
-            if (squares) lds.red[1][r + i][pc] = sq;
-        }
-        if (trans_at >= 0) {
-            const int p = (r & 32) | swap23(r & 31);  // four rows stay consecutive
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const vec4 w = {xv[0][e], xv[1][e], xv[2][e], xv[3][e]};
-                *reinterpret_cast<vec4*>(&lds.t[(pc * 8 + e) * kRow + p]) = w;
-            }
+            if (y) lds.red[0][r][pc] = dot;
+            if (squares) lds.red[1][r][pc] = sq;
         }
     }
     __syncthreads();
-    if (trans_at >= 0) {
-        for (int id = t; id < D * 8; id += 256) {  // 16-byte pieces: unit, fragment (s, md), lane
-            const int u = id / (D * 4);
-            const int f = (id % (D * 4)) >> 6;
-            const int lane = id & 63;
-            const int dim = f % (D / 32) * 32 + (lane & 31);
-            const int pos = u * 32 + f / (D / 32) * 16 + (lane >> 5) * 8;
-            store8(units + u * unit_bytes + (trans_at + f) * 1024 + lane * 16,
-                   *reinterpret_cast<const vec8*>(&lds.t[dim * kRow + pos]));
-        }
-    }
 }
 
 // Largest sqrt of the rows' sums of squares, by the first wave.
-template <typename T, int D> __device__ __forceinline__ float largest_row(const PackLds<T, D>& lds) {
+template <int D> __device__ __forceinline__ float largest_row(const PackLds<D>& lds) {
     float s = 0.0f;
     for (int j = 0; j < D / 8; ++j) s += lds.red[1][threadIdx.x][j];
     s = sqrtf(s);
@@ -155,9 +151,7 @@ template <typename T, int D> __device__ __forceinline__ float largest_row(const 
 // One workgroup per 64-row block of one tensor: dO (with O), Q, K, V.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardArgs a) {
-    constexpr int KT = D / 16;
-    constexpr int64_t kQBytes = q_unit_frags<D>() * 1024, kKvBytes = kv_unit_frags<D>() * 1024;
-    __shared__ __attribute__((aligned(16))) PackLds<T, D> lds;
+    __shared__ PackLds<D> lds;
     const int q_blocks = a.q_units / 2, kv_blocks = a.kv_units / 2;
     const int q_work = a.batch * a.heads * q_blocks, kv_work = a.batch * a.k.heads * kv_blocks;
     const int t = threadIdx.x;
@@ -170,13 +164,13 @@ __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardAr
     auto rows = [&](const View& v) { return v.data + v.row(bh, (int64_t)j * kBlock) * (int64_t)sizeof(T); };
     if (q_side) {
         const int live = a.q_tokens - j * kBlock, last = live - 1;
-        char* units = a.qx + ((int64_t)bh * a.q_units + 2 * j) * kQBytes;
+        char* units = a.qx + ((int64_t)bh * a.q_units + 2 * j) * kUnitBytes<D>;
         if (second) {
-            pack_block<T, D>(lds, rows(a.q), a.q.st, nullptr, 0, live, last, a.head_dim, units, kQBytes, 0, 3 * KT, false);
+            pack_block<T, D>(lds, rows(a.q), a.q.st, nullptr, 0, live, last, a.head_dim, units, false);
             return;
         }
-        pack_block<T, D>(lds, rows(a.dout), a.dout.st, rows(a.o), a.o.st, live, last, a.head_dim, units, kQBytes, KT, 2 * KT,
-                         kScaled<T>);
+        pack_block<T, D>(lds, rows(a.dout), a.dout.st, rows(a.o), a.o.st, live, last, a.head_dim,
+                         units + kOperand<D>, kScaled<T>);
         if (t < kBlock) {
             float delta = 0.0f;
             for (int i = 0; i < D / 8; ++i) delta += lds.red[0][t][i];
@@ -184,11 +178,11 @@ __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardAr
             const int64_t at = (int64_t)bh * a.q_tokens + (int64_t)j * kBlock + t;
             const float dlse = valid && a.dlse ? a.dlse[at] : 0.0f;
             const float nl = valid ? (kScaled<T> ? kShift16 : 0.0f) - a.lse[at] * kLog2e : -__builtin_inff();
-            float* stat = reinterpret_cast<float*>(units + (t >> 5) * kQBytes + 4 * KT * 1024);
-            stat[t & 31] = nl;
-            stat[32 + (t & 31)] = dlse - delta;
+            float* stat = reinterpret_cast<float*>(units + (t >> 5) * kUnitBytes<D> + kGap<D>) + (t & 31);
+            *stat = nl;
+            stat[kOperand<D> / 4] = dlse - delta;
             if constexpr (kScaled<T>) {
-                const float most = largest_row<T, D>(lds);
+                const float most = largest_row<D>(lds);
                 float most_l = fabsf(dlse);
 #pragma unroll
                 for (int o = 32; o > 0; o >>= 1) most_l = fmaxf(most_l, __shfl_xor(most_l, o));
@@ -201,15 +195,15 @@ __global__ __launch_bounds__(256) void attention_backward_pack_kernel(BackwardAr
     } else {
         const int last = a.kv_tokens - j * kBlock - 1;
         const int live = a.length(bh / a.k.heads) - j * kBlock;
-        char* units = a.kx + ((int64_t)bh * a.kv_units + 2 * j) * kKvBytes;
+        char* units = a.kx + ((int64_t)bh * a.kv_units + 2 * j) * kUnitBytes<D>;
         if (!second) {
-            pack_block<T, D>(lds, rows(a.k), a.k.st, nullptr, 0, live, last, a.head_dim, units, kKvBytes, 0, 2 * KT, false);
+            pack_block<T, D>(lds, rows(a.k), a.k.st, nullptr, 0, live, last, a.head_dim, units, false);
             return;
         }
-        pack_block<T, D>(lds, rows(a.v), a.v.st, nullptr, 0, live, last, a.head_dim, units, kKvBytes, KT, -1, kScaled<T>);
+        pack_block<T, D>(lds, rows(a.v), a.v.st, nullptr, 0, live, last, a.head_dim, units + kOperand<D>, kScaled<T>);
         if constexpr (kScaled<T>) {
             if (t < kBlock) {
-                const float most = largest_row<T, D>(lds);
+                const float most = largest_row<D>(lds);
                 if (t == 0) a.v_most[(int64_t)bh * kv_blocks + j] = most;
             }
         }
@@ -240,24 +234,18 @@ __device__ __forceinline__ void wait_copies() {
 // vector register or instruction per copy.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-// Fragments from SPLIT on come from `src1`.
-template <int FRAGS, int SPLIT>
-__device__ __forceinline__ void copy_unit(const char* src0, const char* src1, uint32_t lds_base, int wave,
-                                          uint32_t lane_off) {
+template <int FRAGS>
+__device__ __forceinline__ void copy_unit(const char* src, uint32_t lds_base, int wave, uint32_t lane_off) {
 #pragma unroll
     for (int j = 0; j < (FRAGS + kWaves - 1) / kWaves; ++j) {
         const int f = min(wave + kWaves * j, FRAGS - 1);
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                      :
-                     : "v"(lane_off), "s"((f < SPLIT ? src0 : src1) + f * 1024), "s"(lds_base + f * 1024)
+                     : "v"(lane_off), "s"(src + f * 1024), "s"(lds_base + f * 1024)
                      : "memory", "m0");
     }
 }
 #pragma clang diagnostic pop
-template <int FRAGS>
-__device__ __forceinline__ void copy_unit(const char* src, uint32_t lds_base, int wave, uint32_t lane_off) {
-    copy_unit<FRAGS, FRAGS>(src, src, lds_base, wave, lane_off);
-}
 
 // Pins the own operands to AGPRs (an empty asm with an "a" operand): the matrix
 // core reads its B operand there directly, and the architectural registers are
@@ -275,6 +263,16 @@ template <typename V, int N, int KT> __device__ __forceinline__ void pin_all(V (
 
 template <typename V> __device__ __forceinline__ V lds_frag(const lds_char* p) {
     return __builtin_bit_cast(V, *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(p));
+}
+
+// A fragment of columns: rows 16 s + 8 u + 4 half .. (u = 0, 1) of a lane's dim
+// (swap23 order), p at transposing_at.
+template <typename V> __device__ __forceinline__ V lds_columns(const lds_char* p) {
+    typedef short vec4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) vec4 lds_vec4;
+    const vec4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec4*)p);
+    const vec4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec4*)(p + 128));
+    return __builtin_bit_cast(V, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // log2 of the factor on dS in fp16: of the largest power of two that keeps
@@ -415,18 +413,19 @@ __global__ __launch_bounds__(64) void attention_backward_join_kernel(BackwardArg
 
 // LDS of a workgroup: the streamed units, at width 128 a part of the wave's own
 // values (kValuesInLds), and a few words to share.
+constexpr int kKvStages = 3;  // the unit in use and two on their way
+constexpr int kQStages = 4;   // and the unit before, whose columns are read
 template <int D> constexpr int kv_lds_bytes() {
-    return stages<D>() * q_unit_frags<D>() * 1024 + (kValuesInLds<D> ? kWaves * (D / 16) * 1024 : 0);
+    return kKvStages * kUnitBytes<D> + (kValuesInLds<D> ? kWaves * (D / 16) * 1024 : 0);
 }
-constexpr int kQStages = 3;
-template <int D> constexpr int q_lds_bytes() { return kQStages * kv_unit_frags<D>() * 1024; }
+template <int D> constexpr int q_lds_bytes() { return kQStages * kUnitBytes<D>; }
 
 // ---------------------------------------------------------------- dK, dV
 template <typename T, int D>
 __device__ __forceinline__ void backward_kv(const BackwardArgs& a, int index, lds_char* lds, float (*scratch)[kWaves]) {
     typedef typename Elem<T>::vec8 vec8;
-    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = q_unit_frags<D>(), S = stages<D>(), R = D > 128 && D < 256 ? 8 : 4;
-    constexpr int kBytes = FRAGS * 1024;
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kUnitFrags<D>, S = kKvStages, R = kKvAhead;
+    constexpr int kBytes = kUnitBytes<D>;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const TileWork work = tile_work(a.kv_tiles, index);
@@ -452,19 +451,20 @@ __device__ __forceinline__ void backward_kv(const BackwardArgs& a, int index, ld
     const uint32_t base = (uint32_t)(uintptr_t)lds;
     if (i0 < i1) {
         copy_unit<FRAGS>(unit_of(i0), base, wave, lane * 16);
-        if constexpr (S == 3) copy_unit<FRAGS>(unit_of(i0 + 1), base + kBytes, wave, lane * 16);
+        copy_unit<FRAGS>(unit_of(i0 + 1), base + kBytes, wave, lane * 16);
     }
+    static_assert(4 * KT % R == 0, "the ring goes on into the next unit");
+    const int row_lane = lane_at(half, col), column_lane = transposing_at<D>(lane);
     constexpr int NV = kValuesInLds<D> ? N - 1 : N;
     lds_char* const own_v = lds + S * kBytes + wave * KT * 1024 + lane * 16;
     vec8 kf[N][KT], vf[NV][KT];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const char* own = a.kx + ((int64_t)bh * a.kv_units + min(unit0 + n, a.kv_units - 1)) * (kv_unit_frags<D>() * 1024) +
-                          lane * 16;
+        const char* own = a.kx + ((int64_t)bh * a.kv_units + min(unit0 + n, a.kv_units - 1)) * kBytes + row_lane;
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-            kf[n][t] = load8<vec8>(own + t * 1024);
-            const vec8 x = load8<vec8>(own + (KT + t) * 1024);
+            kf[n][t] = load8<vec8>(own + frag_at<D>(t));
+            const vec8 x = load8<vec8>(own + kOperand<D> + frag_at<D>(t));
             if (n < NV)
                 vf[n][t] = x;
             else
@@ -489,16 +489,23 @@ __device__ __forceinline__ void backward_kv(const BackwardArgs& a, int index, ld
     if (i0 < i1) {
         __builtin_amdgcn_s_waitcnt(kWaitVm0);  // the own operands have landed too: only copies are in flight from here on
         wait_copies();
+        // fragment used j-th: Q rows, dO rows, dO columns, Q columns
+        auto fragment = [&](const lds_char* rows, const lds_char* columns, auto index) __attribute__((always_inline)) {
+            constexpr int j = index, phase = j / KT, t = j % KT, at = phase == 1 || phase == 2 ? kOperand<D> : 0;
+            if constexpr (phase < 2)
+                return lds_frag<vec8>(rows + at + frag_at<D>(t));
+            else
+                return lds_columns<vec8>(columns + at + t % MD * 1024 + t / MD * 256);
+        };
         vec8 ring[R];  // the next fragments, read R steps ahead
-#pragma unroll
-        for (int j = 0; j < R; ++j) ring[j] = lds_frag<vec8>(lds + lane * 16 + j * 1024);
+        unrolled<R>([&](auto j) __attribute__((always_inline)) { ring[j] = fragment(lds + row_lane, lds, j); });
         int buf = 0;
         for (int i = i0; i < i1; ++i) {
             const int next = buf == S - 1 ? 0 : buf + 1;
-            if constexpr (S == 2) copy_unit<FRAGS>(unit_of(i + 1), base + next * kBytes, wave, lane * 16);
-            const lds_char* const u = lds + buf * kBytes + lane * 16;
-            const lds_char* const un = lds + next * kBytes + lane * 16;
-            const lds_char* const stat = lds + buf * kBytes + 4 * KT * 1024 + half * 16;
+            const lds_char* const u = lds + buf * kBytes + row_lane;
+            const lds_char* const uc = lds + buf * kBytes + column_lane;
+            const lds_char* const un = lds + next * kBytes + row_lane;
+            const lds_char* const stat = lds + buf * kBytes + kGap<D> + half * 16;
             pin_all(vf);
             f32x16 s[N], dp[N], nl, nd, zero;
             vec8 p[N][2], ds[N][2], vring[2];
@@ -515,14 +522,14 @@ __device__ __forceinline__ void backward_kv(const BackwardArgs& a, int index, ld
                     if constexpr (phase == 3) dk[n][t % MD] = mfma32(x, ds[n][t / MD], dk[n][t % MD]);
                 }
                 if constexpr (j + R < 4 * KT)
-                    ring[j % R] = lds_frag<vec8>(u + (j + R) * 1024);
-                else if constexpr (S == 3)
-                    ring[j % R] = lds_frag<vec8>(un + (j + R - 4 * KT) * 1024);
+                    ring[j % R] = fragment(u, uc, std::integral_constant<int, j + R>{});
+                else
+                    ring[j % R] = fragment(un, uc, std::integral_constant<int, j + R - 4 * KT>{});
                 if constexpr (kValuesInLds<D> && ((phase == 0 && t >= KT - 2) || (phase == 1 && t < KT - 2)))
                     vring[t % 2] = lds_frag<vec8>(own_v + (phase == 0 ? t - (KT - 2) : t + 2) * 1024);
                 if constexpr (phase == 0 && t >= KT - 4) {  // four rows of dL - delta
                     constexpr int q = t - (KT - 4);
-                    const f32x4 y = lds_frag<f32x4>(stat + 128 + q * 32);
+                    const f32x4 y = lds_frag<f32x4>(stat + kOperand<D> + q * 32);
 #pragma unroll
                     for (int w = 0; w < 4; ++w) nd[4 * q + w] = y[w];
                 }
@@ -554,7 +561,7 @@ __device__ __forceinline__ void backward_kv(const BackwardArgs& a, int index, ld
                     });
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (S == 3 && j == 2 * KT - 1) {
+                if constexpr (j == 2 * KT - 1) {
                     // every wave is past unit i - 1, and unit i + 1 has landed: its buffer is the
                     // first one's to fill and the other may be read ahead
                     wait_copies();
@@ -562,28 +569,25 @@ __device__ __forceinline__ void backward_kv(const BackwardArgs& a, int index, ld
                     __builtin_amdgcn_sched_barrier(0);
                 }
             });
-            if constexpr (S == 2) {
-                wait_copies();
-#pragma unroll
-                for (int j = 0; j < R; ++j) ring[j] = lds_frag<vec8>(un + j * 1024);
-            }
             buf = next;
         }
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // no copy outlives the workgroup's LDS
     }
+    // at width 128 the lane is not held over the loop (its register is needed there)
+    const int lane_out = kValuesInLds<D> ? __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)) : lane;
     const float kfac = a.scale * __builtin_amdgcn_exp2f(-e), vfac = kScaled<T> ? __builtin_amdgcn_exp2f(-kShift16) : 1.0f;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int unit = unit0 + n;
         if (unit >= a.kv_units) continue;
-        const int key = unit * kUnit + col;
+        const int key = unit * kUnit + (lane_out & 31);
         const bool inside = key < a.kv_tokens, live = key < length;
         const int64_t at = inside ? key : 0;
         float* slot = nullptr;
         if (work.slot >= 0) slot = a.kv_part + (((int64_t)work.slot * kWaves + wave) * N + n) * MD * 1024;
-        store_unit<T, MD>(dk[n], kfac, live, slot, reinterpret_cast<T*>(a.dk.data) + a.dk.row(bh, at), inside, a.head_dim, lane);
+        store_unit<T, MD>(dk[n], kfac, live, slot, reinterpret_cast<T*>(a.dk.data) + a.dk.row(bh, at), inside, a.head_dim, lane_out);
         if (slot) slot += (int64_t)a.kv_tiles.parts * a.kv_tiles.rest * kWaves * N * MD * 1024;
-        store_unit<T, MD>(dv[n], vfac, live, slot, reinterpret_cast<T*>(a.dv.data) + a.dv.row(bh, at), inside, a.head_dim, lane);
+        store_unit<T, MD>(dv[n], vfac, live, slot, reinterpret_cast<T*>(a.dv.data) + a.dv.row(bh, at), inside, a.head_dim, lane_out);
     }
 }
 
@@ -591,8 +595,8 @@ __device__ __forceinline__ void backward_kv(const BackwardArgs& a, int index, ld
 template <typename T, int D>
 __device__ __forceinline__ void backward_q(const BackwardArgs& a, int index, lds_char* lds, float (*scratch)[kWaves]) {
     typedef typename Elem<T>::vec8 vec8;
-    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kv_unit_frags<D>(), S = kQStages, R = D <= 128 ? 6 : D == 160 ? 10 : 12;
-    constexpr int kBytes = FRAGS * 1024;
+    constexpr int KT = D / 16, MD = D / 32, N = columns<D>(), FRAGS = kUnitFrags<D>, S = kQStages, R = kQAhead;
+    constexpr int kBytes = kUnitBytes<D>;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const TileWork work = tile_work(a.q_tiles, index);
@@ -606,13 +610,11 @@ __device__ __forceinline__ void backward_q(const BackwardArgs& a, int index, lds
     const int i0 = (int)((int64_t)steps * work.part / work.parts), i1 = (int)((int64_t)steps * (work.part + 1) / work.parts);
     const char* const table = a.kx + (int64_t)kv_bh * a.kv_units * kBytes;
     auto unit_of = [&](int i) { return table + (int64_t)min(i, i1 - 1) * kBytes; };
-    // fragment of the buffer used j-th: K rows, K^T, V rows
-    auto order = [](int j) { return j < KT ? j : j < 2 * KT ? j + KT : j - KT; };
+    static_assert(3 * KT % R == 0, "the ring goes on into the next step");
+    const int row_lane = lane_at(half, col), column_lane = transposing_at<D>(lane);
 
     const uint32_t base = (uint32_t)(uintptr_t)lds;
-    auto copy_step = [&](int i, int b) {
-        copy_unit<FRAGS, 2 * KT>(unit_of(i), unit_of(max(i - 1, i0)), base + b * kBytes, wave, lane * 16);
-    };
+    auto copy_step = [&](int i, int b) { copy_unit<FRAGS>(unit_of(i), base + b * kBytes, wave, lane * 16); };
     if (i0 < i1) {
         copy_step(i0, 0);
         copy_step(i0 + 1, 1);
@@ -621,14 +623,14 @@ __device__ __forceinline__ void backward_q(const BackwardArgs& a, int index, lds
     float nl[N], nd[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const char* own = a.qx + ((int64_t)bh * a.q_units + min(unit0 + n, a.q_units - 1)) * (q_unit_frags<D>() * 1024);
-        const float* stat = reinterpret_cast<const float*>(own + 4 * KT * 1024);
-        nl[n] = stat[col];
-        nd[n] = stat[32 + col];
+        const char* own = a.qx + ((int64_t)bh * a.q_units + min(unit0 + n, a.q_units - 1)) * kBytes;
+        const float* stat = reinterpret_cast<const float*>(own + kGap<D>) + col;
+        nl[n] = *stat;
+        nd[n] = stat[kOperand<D> / 4];
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-            qf[n][t] = load8<vec8>(own + t * 1024 + lane * 16);
-            of[n][t] = load8<vec8>(own + (KT + t) * 1024 + lane * 16);
+            qf[n][t] = load8<vec8>(own + frag_at<D>(t) + row_lane);
+            of[n][t] = load8<vec8>(own + kOperand<D> + frag_at<D>(t) + row_lane);
         }
     }
     float e = 0.0f;  // log2 of dS's factor
@@ -648,22 +650,32 @@ __device__ __forceinline__ void backward_q(const BackwardArgs& a, int index, lds
             for (int v = 0; v < 16; ++v) dq[n][md][v] = 0.0f;
 
     // Step i forms S and dP of unit i and adds unit i - 1 to dQ: dS of i - 1 is formed
-    // beside the products of S, the probabilities of i beside those of dQ.  (The
-    // buffer of step i therefore holds K and V rows of unit i and K^T of i - 1.)
+    // beside the products of S, the probabilities of i beside those of dQ.
     if (i0 < i1) {
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
         wait_copies();
+        // fragment used j-th: K rows of unit i, K columns of i - 1, V rows of i
+        auto fragment = [&](const lds_char* rows, const lds_char* columns, auto index) __attribute__((always_inline)) {
+            constexpr int j = index, phase = j / KT, t = j % KT;
+            if constexpr (phase == 1)
+                return lds_columns<vec8>(columns + t % MD * 1024 + t / MD * 256);
+            else
+                return lds_frag<vec8>(rows + (phase == 2 ? kOperand<D> : 0) + frag_at<D>(t));
+        };
         vec8 ring[R];
-#pragma unroll
-        for (int j = 0; j < R; ++j) ring[j] = lds_frag<vec8>(lds + lane * 16 + order(j) * 1024);
+        unrolled<R>([&](auto j) __attribute__((always_inline)) {
+            ring[j] = fragment(lds + row_lane, lds + (S - 1) * kBytes + column_lane, j);
+        });
         f32x16 s[N], dp[N];
         int buf = 0;
         // first: there is no unit i - 1; last: no unit i
         auto step = [&](int i, auto is_first, auto is_last) __attribute__((always_inline)) {
             constexpr bool first = is_first, last = is_last;
             const int next = buf == S - 1 ? 0 : buf + 1;
-            const lds_char* const u = lds + buf * kBytes + lane * 16;
-            const lds_char* const un = lds + next * kBytes + lane * 16;
+            const lds_char* const u = lds + buf * kBytes + row_lane;
+            const lds_char* const uc = lds + (buf == 0 ? S - 1 : buf - 1) * kBytes + column_lane;  // of unit i - 1
+            const lds_char* const un = lds + next * kBytes + row_lane;
+            const lds_char* const unc = lds + buf * kBytes + column_lane;
             pin_all(qf);
             pin_all(of);
             f32x16 sn[N], zero, start[N];
@@ -684,9 +696,9 @@ __device__ __forceinline__ void backward_q(const BackwardArgs& a, int index, lds
                     if constexpr (phase == 2 && !last) dp[n] = mfma32(x, of[n][t], t == 0 ? start[n] : dp[n]);
                 }
                 if constexpr (j + R < 3 * KT)
-                    ring[j % R] = lds_frag<vec8>(u + order(j + R) * 1024);
+                    ring[j % R] = fragment(u, uc, std::integral_constant<int, j + R>{});
                 else if constexpr (!last)
-                    ring[j % R] = lds_frag<vec8>(un + order(j + R - 3 * KT) * 1024);
+                    ring[j % R] = fragment(un, unc, std::integral_constant<int, j + R - 3 * KT>{});
                 if constexpr (phase == 0 ? !first : phase == 1 && !last && t > 0) {
                     constexpr int part = phase == 0 ? t : t - 1, parts = phase == 0 ? KT : KT - 1;
                     constexpr int from = part * 8 * N / parts, to = (part + 1) * 8 * N / parts;
@@ -712,9 +724,9 @@ __device__ __forceinline__ void backward_q(const BackwardArgs& a, int index, lds
 #pragma unroll
                                 for (int n = 0; n < N; ++n) sn[n][v] = -__builtin_inff();
                     }
-                    // every wave is past step i - 1, and step i + 1's fragments have landed
+                    // every wave is past step i - 1 (and unit i - 2), and unit i + 1 has landed
                     wait_copies();
-                    if constexpr (!last) copy_step(i + 2, buf == 0 ? S - 1 : buf - 1);
+                    if constexpr (!last) copy_step(i + 2, buf ^ 2);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             });
@@ -887,8 +899,8 @@ BackwardPlan plan_backward(int batch, int heads, int kv_heads, int q_tokens, int
     plan_tiles(kv, q, kv_parts, q_parts);
     p.kv_tiles = tiles_of(kv, kv_per_head, kv_parts);
     p.q_tiles = tiles_of(q, q_per_head, q_parts);
-    p.qx_bytes = bh * p.q_units * (4 * (padded / 16) + 1) * 1024;
-    p.kx_bytes = kv_bh * p.kv_units * 3 * (padded / 16) * 1024;
+    p.qx_bytes = bh * p.q_units * (padded / 8 + 1) * 1024;
+    p.kx_bytes = kv_bh * p.kv_units * (padded / 8 + 1) * 1024;
     p.q_most_bytes = scaled ? bh * (p.q_units / 2) * (int64_t)sizeof(float) : 0;
     p.l_most_bytes = p.q_most_bytes;
     p.v_most_bytes = scaled ? kv_bh * (p.kv_units / 2) * (int64_t)sizeof(float) : 0;

@@ -85,15 +85,16 @@ def test_backward_outputs(lib):
 def test_workspace_bytes(lib):
     size = lib.LIB.attn_hip_dense_backward_workspace_bytes
     assert size(2, 1, 4, 2, 6, 9, 64) == 0 and size(0, 1, 4, 3, 6, 9, 64) == 0 and size(0, 1, 4, 2, 6, 9, 4) == 0
-    # [Q][dO][Q^T][dO^T] and 1 KB of row values per 32 queries, [K][V][K^T] per 32 keys
-    unit = 64 * 32 * 2
-    assert size(0, 1, 4, 2, 64, 64, 64) == 4 * 2 * (4 * unit + 1024) + 2 * 2 * 3 * unit
+    # 32 rows of two operands (Q and dO, or K and V) and 1 KB, of which 256 bytes are the rows' values
+    unit = 2 * 64 * 32 * 2 + 1024
+    assert size(0, 1, 4, 2, 64, 64, 64) == 4 * 2 * unit + 2 * 2 * unit
     # fp16 keeps the largest row norms by block too
     assert size(1, 1, 4, 2, 64, 64, 64) == size(0, 1, 4, 2, 64, 64, 64) + 3 * 256
     # many workgroups: no parts; few: fp32 parts of the gradients
     whole = size(0, 4, 64, 64, 128, 128, 128)
-    assert whole == 256 * 4 * ((4 * 8 + 1) * 1024 + 3 * 8 * 1024)
-    assert size(0, 1, 1, 1, 4096, 64, 128) > 128 * (4 * 8 + 1) * 1024 + 2 * 3 * 8 * 1024 + 2 * 64 * 128 * 4
+    unit = 2 * 128 * 32 * 2 + 1024
+    assert whole == 256 * 4 * (unit + unit)
+    assert size(0, 1, 1, 1, 4096, 64, 128) > 128 * unit + 2 * unit + 2 * 64 * 128 * 4
 
 
 def test_python_refusals_without_a_device():
