@@ -351,3 +351,24 @@ def test_many_heads_and_batches(ops):
         angle = angles(turn["inv_freq"], (8,), pos)
         for x, y in zip((q, k), ops.qk_norm_rope(q, k, **turn)):
             _near(y, *norm_rope(x, None, 1e-6, angle, False), str(tuple(x.shape)))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("shape,k_heads", [((1, 3, 1025, 64), 1), ((2, 3, 1025, 128), 3), ((1, 2, 4099, 80), 1),
+                                           ((3, 1, 2999, 256), 2), ((1, 40, 1031, 128), 8)])
+def test_tiles_of_few_heads(ops, dtype, shape, k_heads):
+    """Tiles of 2, 4, 8 and 16 tokens, the last one of a batch entry partly filled; both orders of a tile's rows."""
+    for layout in ("bthd", "bhtd"):
+        q, k = _rows(1, shape, dtype, layout=layout), _rows(2, (shape[0], k_heads, *shape[2:]), dtype, layout=layout)
+        gq, gk = _rows(3, q.shape, dtype, layout=layout), _rows(4, k.shape, dtype, layout=layout)
+        qw, kw = ((torch.rand(shape[3], generator=torch.Generator().manual_seed(i)) + 0.5).cuda() for i in (5, 6))
+        pos = torch.arange(shape[2], device="cuda", dtype=torch.int32)[:, None]
+        turn = {"inv_freq": ops.rope_frequencies((shape[3],), device="cuda"), "axes_dims": (shape[3],), "positions": pos}
+        angle = angles(turn["inv_freq"], (shape[3],), pos)
+        out = ops.qk_norm_rope(q, k, qw, kw, **turn)
+        grads = ops.qk_norm_rope_backward(gq, gk, q, k, qw, kw, **turn)
+        for x, w, g, y, dx, dw in zip((q, k), (qw, kw), (gq, gk), out, grads[:2], grads[2:]):
+            _near(y, *norm_rope(x, w, 1e-6, angle, False), "y")
+            want, error, want_w, error_w = norm_rope_grad(g, x, w, 1e-6, angle, False)
+            _near(dx, want, error, "dx")
+            _near(dw, want_w, error_w, "dw")
