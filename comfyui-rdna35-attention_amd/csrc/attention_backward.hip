@@ -5,25 +5,38 @@
 //   dS = P (dP - delta),  delta_i = sum_d dO_id O_id,
 //   dQ = scale dS K,  dK = scale dS^T Q
 //
-// One pass packs the operands (pack kernels), two kernels form the products:
-// attention_backward_kv_kernel dK and dV (four products), and
-// attention_backward_q_kernel dQ (three).  S and dP are formed in both: with
-// all five distinct products in one kernel, dQ would be summed over key blocks
-// by fp32 atomics, in an order (and with results) that change from run to run.
+// Three launches: attention_backward_pack_kernel writes the operands in units of
+// 32 rows, attention_backward_kernel forms dK and dV (backward_kv, four products)
+// and dQ (backward_q, three), attention_backward_join_kernel adds the fp32 parts of
+// tiles whose streamed side was split (none in a large problem).  S and dP are
+// formed twice: with all five distinct products in one loop, dQ would be summed
+// over key tiles by fp32 atomics, in an order (and with results) that change from
+// run to run, or dS (heads x Tq x Tk) written out and read again.
 //
-// Both kernels are one scheme.  A wave owns 32 N columns (keys or query rows)
+// Both parts are one scheme.  A wave owns 32 N columns (keys or query rows)
 // whose operands it holds in registers as B operands, and streams the other
 // side in units of 32 rows through LDS, shared by the workgroup's four waves:
 //     X[row][column] = sum_d A[row][d] B[column][d]          (S and dP)
 //     G[dim][column] += sum_row A^T[dim][row] X[row][column]   (dK, dV, dQ)
 // The accumulator of the first product is the B operand of the second as it
 // stands (32x32x16: a lane holds one column), with the streamed rows in
-// swap23 order.  The packing kernels write both forms of every streamed operand
-// as 1 KB fragments, so a unit is one contiguous run of memory, copied to LDS
-// without passing through registers, two units ahead (three buffers; one ahead
-// at width 256), and read back without bank conflicts.  Per 32x32 tile of the
+// swap23 order: no probability passes through LDS.  A unit is one contiguous run
+// of memory, copied to LDS without passing through registers, two units ahead;
+// rows and columns are both read from it without bank conflicts.  (Packing the
+// columns as well, for 16-byte reads of both, took 111 us instead of 67 for
+// [2,16,9216,128] against 512 keys, and the main launch 3 to 10 % longer.)  One wave
+// per SIMD: the gradients (256 registers at width 128) and own operands fill the
+// register file.  The order of products, LDS reads and vector instructions is
+// fixed in the source (unrolled, sched_barrier): left to the compiler's scheduler,
+// registers spill or reads stand right before their use.  Per 32x32 tile of the
 // scores at width 128 the matrix core works 1024 (dK, dV) or 768 (dQ) cycles;
 // each fragment read from LDS feeds two tiles.
+//
+// What bounds it: the matrix cores at the clock that their power leaves.
+// [2,16,9216,128] bf16 (seven products, 4.87 TFLOP): 3790 us = 1285 TFLOP/s, on a
+// card where an 8192^3 bf16 library product reaches 1214; the matrix cores are busy in 60 %
+// of the cycles, at 1.84 GHz.  The pack (115 us there) is memory bound: 690 MB at 6.0 TB/s.
+// Small problems are bound by the chain of launches: [1,8,1000,64] 5 (pack) + 19 + 6 (join) us.
 //
 // A gradient dL of the log sums adds P dL to dS: delta - dL takes delta's place.
 // -L (in log2 units) and dL - delta travel with the query rows; the latter is
@@ -808,7 +821,9 @@ int launch_d(int padded, const BackwardArgs& a, hipStream_t stream) {
 // CUs that a small problem leaves idle; it costs a start-up and an fp32 write for
 // each part and the launch that joins them.  plan_tiles takes the numbers of
 // parts with the smallest estimate of the launch's end.  Costs are in quarters
-// of the time of a dK, dV step at width 128 (about 0.45 us).
+// of the time of a dK, dV step at width 128 (about 0.45 us).  Unsplit and split, us, the
+// joining launch included: [1,8,1000,64] 35.5 and 25, [2,16,9216,128] against 512 keys 422
+// and 274, [1,16 over 4,4001,128] 736 and 421.
 struct TileKind {
     int64_t tiles;  // 0: not formed
     int64_t steps;

@@ -733,6 +733,11 @@ def capabilities() -> dict[str, object]:
         "dense_head_dims": GENERIC_HEAD_DIMS,
         "fixed_block_head_dims": (32, 64, 128),
         "fixed_block_dtypes": (torch.bfloat16, torch.float16, torch.float32),
+        # "backward" above is PISA's; exact attention has one
+        "dense_training_head_dims": GENERIC_HEAD_DIMS,
+        "dense_training_dtypes": TRAIN_DTYPES,
+        "rope_head_dims": ROPE_HEAD_DIMS,
+        "rope_dtypes": ROPE_DTYPES,
     }
 
 
@@ -880,8 +885,10 @@ class _NativeNamespace:
 _C = _NativeNamespace()
 
 # these modules use the helpers above
-from .rotary import axial_rope, qk_norm_rope, qk_norm_rope_backward, rope_frequencies  # noqa: E402
-from .dense_training import dense_attention_backward, dense_attention_with_lse  # noqa: E402
+from .rotary import (  # noqa: E402
+    ROPE_DTYPES, ROPE_HEAD_DIMS, axial_rope, qk_norm_rope, qk_norm_rope_backward, rope_frequencies,
+)
+from .dense_training import TRAIN_DTYPES, dense_attention_backward, dense_attention_with_lse  # noqa: E402
 
 __all__ = [
     "BLOCK_SIZE",

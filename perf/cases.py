@@ -12,7 +12,7 @@ and sampling step:
 * ``spatial`` - mi355x_pisa.forward_spatial_bhtd, the 96x96-token image call;
 * ``video``   - mi355x_pisa.generic_forward on a (frames, height, width) grid.
 
-Everything is forward-only: the package has no backward.
+Everything here is forward-only; the training calls are perf/operators.py's.
 """
 from __future__ import annotations
 

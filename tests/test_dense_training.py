@@ -97,6 +97,16 @@ def test_workspace_bytes(lib):
     assert size(0, 1, 1, 1, 4096, 64, 128) > 128 * unit + 2 * unit + 2 * 64 * 128 * 4
 
 
+def test_capabilities_name_the_training_calls():
+    import mi355x_pisa as ops
+
+    caps = ops.capabilities()
+    assert caps["dense_training_dtypes"] == (torch.bfloat16, torch.float16)
+    assert caps["dense_training_head_dims"] == caps["rope_head_dims"] == tuple(range(8, 257, 8))
+    assert caps["rope_dtypes"] == (torch.bfloat16, torch.float16, torch.float32)
+    assert caps["backward"] is False  # PISA's
+
+
 def test_python_refusals_without_a_device():
     import mi355x_pisa as ops
 
