@@ -1151,6 +1151,34 @@ static int check_train(const char* what, int dtype, int batch, int heads, int kv
     return PISA_OK;
 }
 
+// The packed keys and values, then the parts of shared query blocks.
+static int64_t carve_forward_lse(int batch, int heads, int kv_heads, int q_tokens, int kv_tokens, int head_dim,
+                                 void* workspace, pisa::AttnTrainArgs& a) {
+    const int padded = pisa::padded_head_dim(head_dim);
+    const int64_t packed = attn_hip_dense_workspace_bytes(batch, kv_heads, kv_tokens, head_dim);
+    const int64_t bh = (int64_t)batch * heads;
+    a.q_blocks = (q_tokens + pisa::kBlock - 1) / pisa::kBlock;
+    a.kv_blocks = (kv_tokens + pisa::kBlock - 1) / pisa::kBlock;
+    a.parts = pisa::train_parts(padded, bh, a.q_blocks, a.kv_blocks);
+    Carver c(workspace);
+    char* table = c.take<char>(packed);
+    a.kp = table;
+    a.vp = table ? table + packed / 2 : nullptr;
+    if (a.parts > 1) {
+        a.part_out = c.take<float>(pisa::train_part_floats(padded, bh, a.q_blocks, a.parts) * sizeof(float));
+        a.part_lse = c.take<float>(pisa::train_part_lse_floats(bh, a.q_blocks, a.parts) * sizeof(float));
+    }
+    return c.off;
+}
+
+int64_t attn_hip_dense_forward_lse_workspace_bytes(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads,
+                                                   int32_t q_tokens, int32_t kv_tokens, int32_t head_dim) {
+    if (check_train("dense_forward_lse", dtype, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, 1.0f, nullptr)) return 0;
+    pisa::AttnTrainArgs a;
+    memset(&a, 0, sizeof(a));
+    return carve_forward_lse(batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, nullptr, a);
+}
+
 int attn_hip_dense_forward_lse(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens,
                                int32_t kv_tokens, int32_t head_dim, pisa_view q, pisa_view k, pisa_view v, pisa_view out,
                                float* lse, const int32_t* kv_lengths, float scale, void* workspace,
@@ -1162,27 +1190,22 @@ int attn_hip_dense_forward_lse(int32_t dtype, int32_t batch, int32_t heads, int3
         return rc;
     if (!lse || (reinterpret_cast<uintptr_t>(lse) & 3))
         return fail(PISA_ERR_INVALID_ARGUMENT, "lse must be non-null and aligned to 4 bytes");
-    const int64_t need = attn_hip_dense_workspace_bytes(batch, kv_heads, kv_tokens, head_dim);
+    pisa::AttnTrainArgs aa;
+    memset(&aa, 0, sizeof(aa));
+    const int64_t need = carve_forward_lse(batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, workspace, aa);
     if (!workspace_ok(workspace, workspace_bytes, need))
         return fail(PISA_ERR_WORKSPACE, "workspace of %lld bytes required, got %lld", (long long)need,
                     (long long)workspace_bytes);
     if ((rc = check_device())) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int padded = pisa::padded_head_dim(head_dim);
-    const int kv_blocks = (kv_tokens + pisa::kBlock - 1) / pisa::kBlock;
-    char* kp = static_cast<char*>(workspace);
-    char* vp = kp + need / 2;
-    pisa::AttnTrainArgs aa;
-    memset(&aa, 0, sizeof(aa));
+    const int kv_blocks = aa.kv_blocks;
+    char *kp = static_cast<char*>(workspace), *vp = kp + (aa.vp - aa.kp);
     aa.q = to_view(q, heads);
     aa.o = to_out(out, heads);
-    aa.kp = kp;
-    aa.vp = vp;
     aa.qmap = pisa::TokenMap{0, 0, 0};
     aa.q_tokens = q_tokens;
     aa.kv_tokens = kv_tokens;
-    aa.q_blocks = (q_tokens + pisa::kBlock - 1) / pisa::kBlock;
-    aa.kv_blocks = kv_blocks;
     aa.scale_log2 = scale * pisa::kLog2e;
     aa.inv_scale_log2 = 1.0f / aa.scale_log2;
     aa.head_dim = head_dim;

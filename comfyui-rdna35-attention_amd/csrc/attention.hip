@@ -68,14 +68,16 @@ template <bool TRAIN> using ArgsFor = std::conditional_t<TRAIN, AttnTrainArgs, A
 // A batch entry with no key at all gives zero rows and minus infinity.
 // W > 1 (TRAIN): the W waves of a workgroup share one query block, each walking a
 // contiguous part (`wave`) of its chunks, possibly an empty one, and merge
-// through `merge` (W (MD NT 1024 + 64 NT) floats) in a fixed order.
+// through `merge` (W (MD NT 1024 + 64 NT) floats) in a fixed order.  At W = 4 the
+// block may be shared further, by a.parts workgroups: each then writes its own
+// fp32 rows and log sums (log2 units) to its slot, which attention_join_kernel joins.
 template <typename T, int D, int NT, bool SPARSE, bool TAIL, bool PERSIST = false, bool TRAIN = false, int W = 1>
 __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh, int qb, int sub,
                                                 const int32_t* __restrict__ sel,
                                                 const uint32_t* __restrict__ selmask,
                                                 lds_char* lds = nullptr, bool from_lds = false,
                                                 NextBlock next = NextBlock{0, 0, 0, 0}, int wave = 0,
-                                                float* merge = nullptr) {
+                                                float* merge = nullptr, int part = 0) {
     static_assert(D % 32 == 0 && D <= 256, "padded head dim");
     static_assert(NT == 1 || (NT == 2 && D <= 128), "query tiles per wave");
     typedef typename Elem<T>::vec8 vec8;
@@ -189,8 +191,16 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
 
     // ---- chunk list: [0, n_exact) exact blocks, [n_exact, n_chunks) centroid chunks
     const int all_chunks = TRAIN ? (kv_tokens + kBlock - 1) / kBlock : 0;
-    const int first = W > 1 ? wave * all_chunks / W : 0;  // this wave's first chunk
-    const int n_exact = SPARSE ? a.exact : TRAIN ? (W > 1 ? (wave + 1) * all_chunks / W - first : all_chunks) : a.kv_blocks;
+    constexpr bool kParts = W == 4;
+    int share = wave, shares = W;  // this wave's share of the chunks
+    if constexpr (kParts) {
+        share += part * W;
+        shares *= a.parts;
+    }
+    const int first = W > 1 ? (int)((int64_t)share * all_chunks / shares) : 0;
+    const int n_exact = SPARSE ? a.exact
+                        : TRAIN ? (W > 1 ? (int)((int64_t)(share + 1) * all_chunks / shares) - first : all_chunks)
+                                : a.kv_blocks;
     const int n_chunks = n_exact + (TAIL ? a.npad / kBlock : 0);
     const int32_t* my_idx = SPARSE ? sel + ((int64_t)bh * a.q_blocks + qb) * a.exact : nullptr;
     const uint32_t* my_mask = TAIL ? selmask + ((int64_t)bh * a.q_blocks + qb) * a.mask_words : nullptr;
@@ -593,6 +603,8 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
         }
         __syncthreads();
     }
+    int64_t slot = 0;
+    if constexpr (kParts) slot = (((int64_t)bh * a.q_blocks + qb) * (2 / NT) + sub) * a.parts + part;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const float lf = add_xor32(l[nt]);
@@ -602,6 +614,14 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
         if constexpr (TRAIN) {
             if (all_chunks == 0) inv[nt] = 0.0f;
             const int row = qb * kBlock + 32 * (sub + nt) + col;
+            if constexpr (kParts) {
+                if (a.parts > 1) {
+                    if (lf == 0.0f) inv[nt] = 0.0f;  // no chunk in this part
+                    if (half == 0 && wave == 0)
+                        a.part_lse[(slot * NT + nt) * 32 + col] = __builtin_log2f(lf) - nm[nt];
+                    continue;
+                }
+            }
             if (half == 0 && row < a.q_tokens && wave == 0)
                 a.lse[(int64_t)bh * a.q_tokens + row] = all_chunks == 0 ? -__builtin_inff() : (__builtin_log2f(lf) - nm[nt]) * kLn2;
         }
@@ -638,6 +658,20 @@ __device__ __forceinline__ void attention_block(const ArgsFor<TRAIN>& a, int bh,
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[md][nt][4 * g + e] = x[e];
                 }
+            if constexpr (kParts) {
+                if (a.parts > 1) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            f32x4 x;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = o[md][nt][4 * g + e] * inv[nt];
+                            *reinterpret_cast<f32x4*>(a.part_out + (((slot * MD + md) * NT + nt) * 4 + g) * 256 + lane * 4) = x;
+                        }
+                    continue;
+                }
+            }
         }
         f32x16 corr[NT];
 #pragma unroll
@@ -767,13 +801,80 @@ void attention_shared_kernel(AttnTrainArgs a) {
     // the query fragments of D = 256 (QLDS) are read for the last time before the merge
     __shared__ __attribute__((aligned(1024))) char buf[kMerge > kQuery ? kMerge : kQuery];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int work = xcd_remap(blockIdx.x, gridDim.x);
+    int work = xcd_remap(blockIdx.x, gridDim.x), part = 0;
+    if constexpr (W == 4) {
+        part = work % a.parts;
+        work /= a.parts;
+    }
     const int block_work = work / SUBS;
     const int bh = block_work / a.q_blocks;
     attention_block<T, D, NT, false, false, false, true, W>(
         a, bh, block_work - bh * a.q_blocks, work - block_work * SUBS, nullptr, nullptr,
         kQuery ? (lds_char*)buf + wave * (D / 16) * 1024 : nullptr, false, NextBlock{0, 0, 0, 0}, wave,
-        reinterpret_cast<float*>(buf));
+        reinterpret_cast<float*>(buf), part);
+}
+
+// Joins the parts of a query block's rows in order: weights 2^(lse of the part - the
+// largest), one wave per (work item, 32 dims, 32 rows).
+template <typename T, int D>
+__global__ __launch_bounds__(64) void attention_join_kernel(AttnTrainArgs a) {
+    constexpr int NT = D <= 128 ? 2 : 1, SUBS = 2 / NT, MD = D / 32;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x, half = lane >> 5, col = lane & 31;
+    const int nt = blockIdx.x % NT;
+    const int md = blockIdx.x / NT % MD;
+    const int item = blockIdx.x / (NT * MD);
+    const int block_work = item / SUBS;
+    const int bh = block_work / a.q_blocks;
+    const int row = (block_work - bh * a.q_blocks) * kBlock + 32 * (item - block_work * SUBS + nt) + col;
+    const int64_t slot = (int64_t)item * a.parts;
+    constexpr int kBatch = 8;  // parts whose loads go out together
+    const float* lse = a.part_lse + (slot * NT + nt) * 32 + col;
+    float top = -__builtin_inff();
+    for (int p0 = 0; p0 < a.parts; p0 += kBatch) {
+        float y[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) y[i] = lse[min(p0 + i, a.parts - 1) * NT * 32];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) top = __builtin_elementwise_maximum(top, y[i]);
+    }
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+    f32x16 x;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[v] = 0.0f;
+    const float* src = a.part_out + (slot * MD * NT + md * NT + nt) * 1024 + lane * 4;
+    for (int p0 = 0; p0 < a.parts; p0 += kBatch) {
+        float w[kBatch];
+        f32x4 y[kBatch][4];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int p = min(p0 + i, a.parts - 1);
+            w[i] = lse[p * NT * 32];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) y[i][g] = *reinterpret_cast<const f32x4*>(src + (int64_t)p * MD * NT * 1024 + g * 256);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // all of them before the first use
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (p0 + i >= a.parts) break;
+            w[i] = __builtin_amdgcn_exp2f(w[i] - base);
+            sum += w[i];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) x[v] = fmaf(y[i][v / 4][v % 4], w[i], x[v]);
+        }
+    }
+    if (row >= a.q_tokens) return;
+    if (md == 0 && half == 0) a.lse[(int64_t)bh * a.q_tokens + row] = (__builtin_log2f(sum) + base) * kLn2;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = reinterpret_cast<T*>(a.o.data) + a.o.row(bh, row);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int d = md * 32 + 8 * g + 4 * half;
+        const vec4 y = {from_f32<T>(x[4 * g] * inv), from_f32<T>(x[4 * g + 1] * inv), from_f32<T>(x[4 * g + 2] * inv),
+                        from_f32<T>(x[4 * g + 3] * inv)};
+        if (d < a.head_dim) *reinterpret_cast<vec4*>(out + d) = y;
+    }
 }
 
 // Persistent variant (D = 128, head dim 128, a grid that splits evenly into the
@@ -1018,19 +1119,31 @@ static int launch_train_d(const AttnTrainArgs& a, int bh_count, hipStream_t stre
     auto cost = [&](int w) {
         return ((int64_t)items * w + simds - 1) / simds * ((a.kv_blocks + w - 1) / w + (w > 1 ? 4 : 0));
     };
-    if (items < simds && cost(4) < cost(1) && cost(4) <= cost(2)) {
-        hipLaunchKernelGGL((attention_shared_kernel<T, D, 4>), dim3(items), dim3(256), 0, stream, a);
-        return pisa_host::check_launch("attention_shared_kernel");
+    if (a.parts > 1) {
+        hipLaunchKernelGGL((attention_shared_kernel<T, D, 4>), dim3(items * a.parts), dim3(256), 0, stream, a);
+        if (int rc = pisa_host::check_launch("attention_shared_kernel")) return rc;
+        hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3(items * (D <= 128 ? 2 : 1) * (D / 32)), dim3(64), 0, stream, a);
+        return pisa_host::check_launch("attention_join_kernel");
     }
-    if (items < simds && cost(2) < cost(1)) {
-        hipLaunchKernelGGL((attention_shared_kernel<T, D, 2>), dim3(items), dim3(128), 0, stream, a);
-        return pisa_host::check_launch("attention_shared_kernel");
+    if constexpr (D == 64) {
+        return launch_attention_d64_train(std::is_same<T, bf16_t>::value ? PISA_DTYPE_BF16 : PISA_DTYPE_F16, a, bh_count,
+                                          stream);
+    } else {
+        if (items < simds && cost(4) < cost(1) && cost(4) <= cost(2)) {
+            hipLaunchKernelGGL((attention_shared_kernel<T, D, 4>), dim3(items), dim3(256), 0, stream, a);
+            return pisa_host::check_launch("attention_shared_kernel");
+        }
+        if (items < simds && cost(2) < cost(1)) {
+            hipLaunchKernelGGL((attention_shared_kernel<T, D, 2>), dim3(items), dim3(128), 0, stream, a);
+            return pisa_host::check_launch("attention_shared_kernel");
+        }
+        return launch_attention_t<T, D, false, false, true>(a, bh_count, stream);
     }
-    return launch_attention_t<T, D, false, false, true>(a, bh_count, stream);
 }
 template <typename T>
 static int launch_train_t(int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
     switch (padded) {
+        case 64: return launch_train_d<T, 64>(a, bh_count, stream);
         case 96: return launch_train_d<T, 96>(a, bh_count, stream);
         case 128: return launch_train_d<T, 128>(a, bh_count, stream);
         case 160: return launch_train_d<T, 160>(a, bh_count, stream);
@@ -1039,8 +1152,37 @@ static int launch_train_t(int padded, const AttnTrainArgs& a, int bh_count, hipS
         default: return pisa_host::fail(PISA_ERR_UNSUPPORTED, "training attention: padded head dim %d", padded);
     }
 }
+
+// Workgroups that share the keys of a query block (1: none): few query blocks
+// against long key lists, where even four waves a block leave most CUs idle.  In
+// chunks' times (about 1.5 us): a wave's chunks, four for the merge in the workgroup, six
+// and one for every eight parts for the joining launch.  Head dims up to 64 have eight
+// waves a block without it.  Unsplit and split, us, both launches: 26 heads of one query
+// against 8369 keys of 72 dims 56.8 and 25, [1,8,1,128] against 9216 53.8 and 18,
+// [1,11,194,128] against 5433 38.1 and 22, [1,8,1,64] against 9216 34.4 and 14.
+int train_parts(int padded, int64_t bh_count, int q_blocks, int kv_blocks) {
+    constexpr int kMostParts = 32, kCus = 256;
+    const int64_t items = bh_count * q_blocks * (padded <= 128 ? 1 : 2);
+    const int waves = padded == 64 ? 8 : 4;
+    int best = 1, cost = (kv_blocks + waves - 1) / waves + 4;
+    for (int p = 2; p <= kMostParts && items * p <= kCus; ++p) {
+        const int c = (kv_blocks + 4 * p - 1) / (4 * p) + 4 + 6 + p / 8;
+        if (c < cost) {
+            cost = c;
+            best = p;
+        }
+    }
+    return best;
+}
+// Floats of the parts' rows and of their log sums.
+int64_t train_part_floats(int padded, int64_t bh_count, int q_blocks, int parts) {
+    return parts > 1 ? bh_count * q_blocks * kBlock * parts * padded : 0;
+}
+int64_t train_part_lse_floats(int64_t bh_count, int q_blocks, int parts) {
+    return parts > 1 ? bh_count * q_blocks * kBlock * parts : 0;
+}
+
 int launch_attention_train(int dtype, int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream) {
-    if (padded == 64) return launch_attention_d64_train(dtype, a, bh_count, stream);
     if (dtype == PISA_DTYPE_BF16) return launch_train_t<bf16_t>(padded, a, bh_count, stream);
     return launch_train_t<f16_t>(padded, a, bh_count, stream);
 }

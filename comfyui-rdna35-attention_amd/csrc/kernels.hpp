@@ -168,6 +168,8 @@ struct AttnTrainArgs : AttnArgs {
     float* lse;                 // [BH][q_tokens]
     const int32_t* kv_lengths;  // [B] or null
     int kv_group;               // query heads per key head
+    int parts;                  // workgroups to a query block (train_parts)
+    float *part_out, *part_lse; // their rows and log sums (parts > 1)
 };
 
 struct LayoutArgs {
@@ -240,6 +242,9 @@ struct PackMeans {
 int launch_kv_pack_lengths(int dtype, int padded, int head_dim, const View& k, const View& v, const int32_t* kv_lengths,
                            int kv_tokens, int kv_blocks, int bh_count, char* kp, char* vp, hipStream_t stream);
 // Dense attention that also writes the rows' log sums (attention_train.hip).
+int train_parts(int padded, int64_t bh_count, int q_blocks, int kv_blocks);
+int64_t train_part_floats(int padded, int64_t bh_count, int q_blocks, int parts);
+int64_t train_part_lse_floats(int64_t bh_count, int q_blocks, int parts);
 int launch_attention_train(int dtype, int padded, const AttnTrainArgs& a, int bh_count, hipStream_t stream);
 int launch_kv_pack_means(int dtype, int padded, int head_dim, const View& k, const View& v, TokenMap map, int kv_tokens,
                          int kv_blocks, int bh_count, char* kp, char* vp, const PackMeans& m, hipStream_t stream);

@@ -148,6 +148,7 @@ _SIGNATURES = {
         ctypes.c_int,
         [_i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, _f32, _i32, PisaMask, _vp],
     ),
+    "attn_hip_dense_forward_lse_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "attn_hip_dense_forward_lse": (
         ctypes.c_int,
         [_i32, _i32, _i32, _i32, _i32, _i32, _i32, PisaView, PisaView, PisaView, PisaView, _vp, _vp, _f32, _vp, _i64, _vp],

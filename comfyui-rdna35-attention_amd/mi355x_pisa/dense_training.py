@@ -65,12 +65,13 @@ def _forward_kernel(q, k, v, scale: float, kv_lengths):
     kv_heads, kv_tokens = k.shape[1], k.shape[2]
     out = _heads_last(q)
     lse = torch.empty((batch, heads, q_tokens), dtype=torch.float32, device=q.device)
+    code = dtype_code(q.dtype)
     with on_device(q.device):
-        ws_bytes = LIB.attn_hip_dense_workspace_bytes(batch, kv_heads, kv_tokens, head_dim)
+        ws_bytes = LIB.attn_hip_dense_forward_lse_workspace_bytes(code, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
         check(
             LIB.attn_hip_dense_forward_lse(
-                dtype_code(q.dtype), batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, view4(q), view4(k), view4(v),
+                code, batch, heads, kv_heads, q_tokens, kv_tokens, head_dim, view4(q), view4(k), view4(v),
                 view4(out), lse.data_ptr(), ptr(kv_lengths), scale, workspace.data_ptr(), ws_bytes, stream_of(q.device),
             ),
             "attn_hip_dense_forward_lse",

@@ -351,3 +351,49 @@ def test_refusals_on_the_device(ops):
     refused_back(ValueError, "grad_lse must be", grad_lse=lse[:1])
     refused_back(TypeError, "lse must be", lse=None)
     refused_back(TypeError, "grad_out must be", grad_out=1.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape,lengths,split", [
+    ((1, 8, 8, 1, 9216, 128), None, True),
+    ((2, 3, 1, 1, 8369, 72), [8369, 70], True),  # entry 1: most parts without a key
+    ((1, 4, 2, 130, 4100, 64), None, False),       # eight waves a block without a join are as fast
+    ((2, 2, 2, 2, 3400, 40), [0, 3399], False),
+    ((1, 4, 2, 130, 8100, 64), None, True),
+    ((2, 2, 2, 2, 7000, 40), [0, 6999], True),     # entry 0: every part without a key
+    ((1, 3, 3, 65, 2999, 160), None, True),
+    ((2, 1, 1, 40, 2500, 256), [65, 2500], True),
+    ((1, 16, 4, 7, 5000, 192), [4990], True),
+])
+def test_few_queries_against_long_key_lists(ops, dtype, shape, lengths, split):
+    """A query block shared by several workgroups and joined."""
+    import mi355x_pisa._lib as lib
+
+    b, h, hk, tq, tk, d = shape
+    size = lib.LIB.attn_hip_dense_forward_lse_workspace_bytes
+    packed = lib.LIB.attn_hip_dense_workspace_bytes(b, hk, tk, d)
+    assert (size(0, b, h, hk, tq, tk, d) > packed + 2 * b * h * 64 * d * 4) == split  # two parts at least
+    assert size(0, b, h, hk, 9216, tk, d) == packed
+    call = _inputs(dtype, shape)
+    first = _check(ops, *call, shape[5] ** -0.5, _lengths(lengths))
+    out, lse = ops.dense_attention_with_lse(*call[:3], shape[5] ** -0.5, kv_lengths=_lengths(lengths))
+    assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+
+
+def test_shared_query_blocks_replay_in_a_graph(ops):
+    q, k, v, _ = _inputs(BF16, (1, 4, 2, 3, 4000, 128))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            want = ops.dense_attention_with_lse(q, k, v, 0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = ops.dense_attention_with_lse(q, k, v, 0.1)
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        k.mul_(-1 - i)  # eager work between the replays
+        want = ops.dense_attention_with_lse(q, k, v, 0.1)
+        torch.cuda.synchronize()
