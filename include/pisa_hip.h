@@ -341,6 +341,11 @@ PISA_HIP_EXPORT int attn_hip_fixed_block_forward_masked(int32_t dtype, int32_t b
 
 /* ---- training: exact attention and its backward pass ---------------------- */
 
+/* Bytes of workspace attn_hip_dense_forward_lse needs (0 for problems it refuses). */
+PISA_HIP_EXPORT int64_t attn_hip_dense_forward_lse_workspace_bytes(int32_t dtype, int32_t batch, int32_t heads,
+                                                   int32_t kv_heads, int32_t q_tokens, int32_t kv_tokens,
+                                                   int32_t head_dim);
+
 /*
  * attn_hip_dense_forward that also writes lse [B*H, Tq] fp32, the natural
  * logarithm of each row's sum of exponentials of the scaled scores.
@@ -349,12 +354,9 @@ PISA_HIP_EXPORT int attn_hip_fixed_block_forward_masked(int32_t dtype, int32_t b
  *               masked (values are taken into [0, Tk]); what stands in them is
  *               not used.  With no key left a row is 0 and its lse minus infinity
  * Every view is 16-byte aligned with strides a multiple of 8 elements; the
- * workspace is of attn_hip_dense_forward_lse_workspace_bytes.
+ * workspace has attn_hip_dense_forward_lse_workspace_bytes.
  * No counterpart in the reference, which is forward-only.
  */
-PISA_HIP_EXPORT int64_t attn_hip_dense_forward_lse_workspace_bytes(int32_t dtype, int32_t batch, int32_t heads,
-                                                   int32_t kv_heads, int32_t q_tokens, int32_t kv_tokens,
-                                                   int32_t head_dim);
 PISA_HIP_EXPORT int attn_hip_dense_forward_lse(int32_t dtype, int32_t batch, int32_t heads, int32_t kv_heads,
                                int32_t q_tokens, int32_t kv_tokens, int32_t head_dim, pisa_view q, pisa_view k,
                                pisa_view v, pisa_view out, float* lse, const int32_t* kv_lengths, float scale,
