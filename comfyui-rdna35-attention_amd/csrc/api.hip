@@ -1212,12 +1212,16 @@ int attn_hip_dense_forward_lse(int32_t dtype, int32_t batch, int32_t heads, int3
     aa.lse = lse;
     aa.kv_lengths = kv_lengths;
     aa.kv_group = heads / kv_heads;
-    const pisa::View kv = to_view(k, kv_heads), vv = to_view(v, kv_heads);
+    const pisa::KvRows kv{to_view(k, kv_heads), to_view(v, kv_heads)};
     const int kv_bh = batch * kv_heads;
+    if (aa.parts == 1 && pisa::train_rows_in_place(padded, aa, kv, batch * heads) &&
+        !views_touch(out, q_tokens, k, kv_tokens, batch, heads, head_dim) &&
+        !views_touch(out, q_tokens, v, kv_tokens, batch, heads, head_dim))
+        return pisa::launch_attention_rows_train(dtype, padded, aa, kv, batch * heads, st);
     if (kv_lengths)
-        rc = pisa::launch_kv_pack_lengths(dtype, padded, head_dim, kv, vv, kv_lengths, kv_tokens, kv_blocks, kv_bh, kp, vp, st);
+        rc = pisa::launch_kv_pack_lengths(dtype, padded, head_dim, kv.k, kv.v, kv_lengths, kv_tokens, kv_blocks, kv_bh, kp, vp, st);
     else
-        rc = pisa::launch_kv_pack(dtype, padded, head_dim, kv, vv, aa.qmap, kv_tokens, kv_blocks, kv_bh, kp, vp, st);
+        rc = pisa::launch_kv_pack(dtype, padded, head_dim, kv.k, kv.v, aa.qmap, kv_tokens, kv_blocks, kv_bh, kp, vp, st);
     if (rc) return rc;
     return pisa::launch_attention_train(dtype, padded, aa, batch * heads, st);
 }

@@ -44,8 +44,9 @@ constexpr int kRawFlags = 0x00020000;  // untyped 32-bit buffer data format
 // values, from two rows each): dense_rows_in_place says when that is the better
 // trade.  Width 128 exists in this form only (340 registers, one wave per SIMD).
 //
-// TRAIN (dense, packed): grouped key heads, a key count per batch entry and the
-// rows' log sums as an output, as in attention.hip.
+// TRAIN (dense): grouped key heads, a key count per batch entry and the rows' log
+// sums as an output, as in attention.hip.  Read in place, a head's rows end with
+// its last live key, so what stands in masked keys reads as zero.
 template <bool TRAIN> using ArgsFor = std::conditional_t<TRAIN, AttnTrainArgs, AttnArgs>;
 
 template <typename T, int D, bool SPARSE, bool TAIL, int W, bool DIRECT, bool TRAIN = false>
@@ -53,7 +54,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D <= 64 
 void attention_parts_kernel(ArgsFor<TRAIN> a, KvRows kv, const int32_t* __restrict__ sel,
                             const uint32_t* __restrict__ selmask) {
     static_assert(!DIRECT || (!SPARSE && !TAIL), "rows are read in place by the dense kernel only");
-    static_assert(!TRAIN || (!SPARSE && !TAIL && !DIRECT), "the training forward is dense and packed");
+    static_assert(!TRAIN || (!SPARSE && !TAIL), "the training forward is dense");
     static_assert(D == 64 || (D == 128 && DIRECT), "packed tables of other widths: attention.hip");
     constexpr int KT = D / 16;  // 16-deep k-steps of the score products
     constexpr int MD = D / 32;  // 32-dim output tiles
@@ -148,11 +149,11 @@ void attention_parts_kernel(ArgsFor<TRAIN> a, KvRows kv, const int32_t* __restri
     // past the last row (or past its last dim) reads as zero.
     const int k_row = DIRECT ? (int)kv.k.st * 2 : 0, v_row = DIRECT ? (int)kv.v.st * 2 : 0;  // bytes
     const __amdgpu_buffer_rsrc_t kr_rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)(DIRECT ? kv.k.data + kv.k.row(bh, 0) * 2 : a.kp), (short)0,
-        DIRECT ? (a.kv_tokens - 1) * k_row + a.head_dim * 2 : 0, kRawFlags);
+        (void*)(DIRECT ? kv.k.data + kv.k.row(kv_bh, 0) * 2 : a.kp), (short)0,
+        !DIRECT || (TRAIN && kv_tokens == 0) ? 0 : (kv_tokens - 1) * k_row + a.head_dim * 2, kRawFlags);
     const __amdgpu_buffer_rsrc_t vr_rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)(DIRECT ? kv.v.data + kv.v.row(bh, 0) * 2 : a.vp), (short)0,
-        DIRECT ? (a.kv_tokens - 1) * v_row + a.head_dim * 2 : 0, kRawFlags);
+        (void*)(DIRECT ? kv.v.data + kv.v.row(kv_bh, 0) * 2 : a.vp), (short)0,
+        !DIRECT || (TRAIN && kv_tokens == 0) ? 0 : (kv_tokens - 1) * v_row + a.head_dim * 2, kRawFlags);
     const bool all_dims = a.head_dim >= D;
 
     auto is_tail = [&](int x) { return TAIL && min(x, n_chunks - 1) >= n_exact; };
@@ -590,6 +591,26 @@ int launch_attention_d64_train(int dtype, const AttnTrainArgs& a, int bh_count, 
     const KvRows none{};
     return dtype == PISA_DTYPE_BF16 ? launch_t<bf16_t, 64, false, false, false, true>(a, none, bh_count, stream)
                                     : launch_t<f16_t, 64, false, false, false, true>(a, none, bh_count, stream);
+}
+
+// The training forward's packed calls above width 64 split their blocks too
+// (attention_shared_kernel), so in place wins with few chunks only.  Packed /
+// in place, us, both launches: [2,13,19,128] 10.2 / 6.4, [2,8,512,128] 16.5 / 14.0,
+// [1,8,1000,128] 20.5 / 19.6, [1,8,2048,128] 29.4 / 33.4, [2,10,1024,80] 23.2 / 26.6;
+// width 64 [1,8,1000,64] 16.3 / 13.7.
+bool train_rows_in_place(int padded, const AttnTrainArgs& a, const KvRows& kv, int bh_count) {
+    const int64_t blocks = (int64_t)bh_count * a.q_blocks, cus = simd_count() > 0 ? simd_count() / 4 : 256;
+    if (padded > 64 && (blocks + cus - 1) / cus * a.kv_blocks > 16) return false;
+    return dense_rows_in_place(padded, a, kv, bh_count);
+}
+
+int launch_attention_rows_train(int dtype, int padded, const AttnTrainArgs& a, const KvRows& kv, int bh_count,
+                                hipStream_t stream) {
+    if (padded == 64)
+        return dtype == PISA_DTYPE_BF16 ? launch_t<bf16_t, 64, false, false, true, true>(a, kv, bh_count, stream)
+                                        : launch_t<f16_t, 64, false, false, true, true>(a, kv, bh_count, stream);
+    return dtype == PISA_DTYPE_BF16 ? launch_t<bf16_t, 128, false, false, true, true>(a, kv, bh_count, stream)
+                                    : launch_t<f16_t, 128, false, false, true, true>(a, kv, bh_count, stream);
 }
 
 int launch_attention_d64(int dtype, bool sparse, const AttnArgs& a, int bh_count, hipStream_t stream) {

@@ -222,6 +222,9 @@ struct KvRows {
 };
 bool dense_rows_in_place(int padded, const AttnArgs& a, const KvRows& kv, int bh_count);
 int launch_attention_rows(int dtype, int padded, const AttnArgs& a, const KvRows& kv, int bh_count, hipStream_t stream);
+bool train_rows_in_place(int padded, const AttnTrainArgs& a, const KvRows& kv, int bh_count);
+int launch_attention_rows_train(int dtype, int padded, const AttnTrainArgs& a, const KvRows& kv, int bh_count,
+                                hipStream_t stream);
 // Packed key / value blocks of width `padded` (dims >= head_dim and rows >= kv_tokens are zero);
 // block j row r is token map(64 j + r).
 int launch_kv_pack(int dtype, int padded, int head_dim, const View& k, const View& v, TokenMap map, int kv_tokens,

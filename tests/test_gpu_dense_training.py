@@ -397,3 +397,22 @@ def test_shared_query_blocks_replay_in_a_graph(ops):
         k.mul_(-1 - i)  # eager work between the replays
         want = ops.dense_attention_with_lse(q, k, v, 0.1)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("layout", ["bthd", "bhtd", "fused"])
+@pytest.mark.parametrize("shape,lengths", [
+    ((2, 4, 2, 65, 129, 64), [129, 0]),
+    ((2, 4, 2, 65, 129, 128), [1, 64]),
+    ((1, 6, 3, 130, 300, 72), [299]),
+    ((1, 8, 8, 200, 1000, 40), None),
+    ((3, 2, 1, 1, 500, 104), [500, 63, 65]),
+])
+def test_small_calls_in_place(ops, dtype, layout, shape, lengths):
+    """Keys and values read where they are: NaN beside every row (fused) and in masked keys."""
+    q, k, v, g = _inputs(dtype, shape, layout)
+    if lengths is not None:
+        for i, n in enumerate(lengths):
+            k[i, :, n:] = math.nan
+            v[i, :, n:] = math.inf
+    _check(ops, q, k, v, g, shape[5] ** -0.5, _lengths(lengths))
