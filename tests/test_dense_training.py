@@ -97,6 +97,19 @@ def test_workspace_bytes(lib):
     assert size(0, 1, 1, 1, 4096, 64, 128) > 128 * unit + 2 * unit + 2 * 64 * 128 * 4
 
 
+def test_forward_workspace_bytes(lib):
+    size, packed = lib.LIB.attn_hip_dense_forward_lse_workspace_bytes, lib.LIB.attn_hip_dense_workspace_bytes
+    assert size(2, 1, 4, 2, 6, 9, 64) == 0 and size(0, 1, 4, 3, 6, 9, 64) == 0 and size(0, 1, 4, 2, 6, 9, 4) == 0
+    assert size(0, 2, 16, 4, 9216, 512, 128) == packed(2, 4, 512, 128)
+    assert size(0, 1, 300, 300, 1, 9216, 128) == packed(1, 300, 9216, 128)  # as many query blocks as CUs: not shared
+    # a query block shared by several workgroups: 64 rows of 128 dims and a log sum each
+    parts, rest = divmod(size(0, 1, 1, 1, 64, 9216, 128) - packed(1, 1, 9216, 128), 64 * 128 * 4 + 64 * 4)
+    assert 2 <= parts <= 32 and rest == 0
+    need = size(1, 1, 1, 1, 64, 9216, 128)
+    assert _forward(lib, dtype=1, heads=1, kv_heads=1, q_tokens=64, kv_tokens=9216, dim=128, held=need - 1) == 3
+    assert b"workspace" in lib.LIB.pisa_hip_last_error()
+
+
 def test_capabilities_name_the_training_calls():
     import mi355x_pisa as ops
 
